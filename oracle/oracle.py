@@ -33,7 +33,7 @@ def _p(a: np.ndarray):
 def build(with_ref: bool = True) -> None:
     """Build liboracle.so and, when the reference checkout is present, _ref/."""
     subprocess.run(["make", "-s", "-C", str(ORACLE_DIR), "all"], check=True)
-    if with_ref and REF_SRC.is_dir():
+    if with_ref and (REF_SRC / "src" / "wav2vec2.cpp").is_file():
         subprocess.run(["make", "-s", "-C", str(ORACLE_DIR), "ref", f"REF={REF_SRC}"], check=True)
 
 
