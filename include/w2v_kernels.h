@@ -201,6 +201,85 @@ int w2v_attention(const void* qkv, void* out, const long long* off, const int* T
 int w2v_ctc_greedy(const float* logits, const long long* off, const int* T, int n_utt, int V,
                    int* ids, int* spans, int* n_spans, int max_T, void* stream);
 
+/* Low-rank adapters of many utterances beside a shared projection:
+ *   C[r] = epi(W A[r] + bias + s_a lora_b[a] (lora_a[a] A[r])),  a = adapter[u]
+ * for the rows off[u] .. off[u]+T[u] of utterance u.  Rows of no utterance,
+ * and of an utterance whose adapter is outside 0 .. n_adapters-1 (-1, say),
+ * get the projection alone.  No counterpart in the reference (one set of
+ * weights per process).
+ *   A: fp16 [M, K] rows, lda elements apart (lda >= K, a multiple of 8; K % 64 == 0).
+ *   W: fp16 [N, K] rows (w2v_gemm_f16_lora) or the planes of w2v_repack_q
+ *      (w2v_gemm_q_lora; Bq, Bs, ld_s and gguf_type as w2v_gemm_q).
+ *   C, ldc, bias, resid, ldr, epilogue: as w2v_gemm_f16, any epilogue but
+ *      W2V_EPI_F32_RESID_LN; resid may alias C.
+ *   lora_a: fp16 [n_adapters][rank][K]; lora_b: fp16 [n_adapters][N][rank];
+ *      lora_scale: fp32 [n_adapters] or NULL (1).  rank: a multiple of 8, at
+ *      most 128 (pad an adapter of another rank with zeros).
+ *   off, T, adapter: device arrays of n_utt entries; off[u+1] >= off[u] + T[u],
+ *      T[u] <= 0 is an utterance without rows.  n_utt == 0: no adapters.
+ *   workspace: device memory of w2v_lora_workspace_bytes(M, n_utt, rank)
+ *      bytes, 128-byte aligned, not shared by calls that may overlap.
+ *      W2V_ERR_CAPACITY when it is too small.
+ * A, W, lora_a, lora_b (and Bs) 16-byte aligned.  s_a lora_a[a] A[r] is held
+ * in fp16 (as two numbers, value and remainder, for the fp32 epilogues): its
+ * magnitude must stay below 65504. */
+long long w2v_lora_workspace_bytes(long long M, int n_utt, int rank);
+int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long long M, const void* B, int N, void* C,
+                      long long ldc, const float* bias, const float* resid, long long ldr, int epilogue,
+                      const void* lora_a, const void* lora_b, const float* lora_scale, int n_adapters, int rank,
+                      const long long* off, const int* T, const int* adapter, int n_utt, void* workspace,
+                      long long workspace_bytes, int* err, void* stream);
+int w2v_gemm_q_lora(const void* A, long long lda, long long K, long long M, const void* Bq, const void* Bs,
+                    long long ld_s, int gguf_type, int N, void* C, long long ldc, const float* bias,
+                    const float* resid, long long ldr, int epilogue, const void* lora_a, const void* lora_b,
+                    const float* lora_scale, int n_adapters, int rank, const long long* off, const int* T,
+                    const int* adapter, int n_utt, void* workspace, long long workspace_bytes, int* err,
+                    void* stream);
+
+/* Matrix products grouped by utterance (output heads per language, routed
+ * experts): C[r] = epi(B[g] A[r] + bias[g]), g = group[u], for the rows
+ * off[u] .. off[u]+T[u] of utterance u (a run of rows sorted by expert is an
+ * "utterance" whose group is the expert).  Rows of no utterance, and of an
+ * utterance whose group is outside 0 .. n_groups-1, are left as they were.
+ * No counterpart in the reference.
+ *   A, lda, K, M, C, ldc, resid, ldr, epilogue: as w2v_gemm_f16_lora.
+ *   B: fp16 [n_groups][N][K], 16-byte aligned; bias: fp32 [n_groups][N] or NULL.
+ *   off, T, group: device arrays of n_utt entries, off[u+1] >= off[u] + T[u]. */
+int w2v_gemm_grouped_f16(const void* A, long long lda, long long K, long long M, const void* B, int n_groups, int N,
+                         void* C, long long ldc, const float* bias, const float* resid, long long ldr, int epilogue,
+                         const long long* off, const int* T, const int* group, int n_utt, int* err, void* stream);
+
+/* CTC prefix beam search on device logits (the search of
+ * wav2vec2_b200_ctc_beam_search, src/ops.h:151-251), the n_best most likely
+ * hypotheses of every utterance, with the beams held in `state` so that the
+ * frames may come in pieces (a live stream, down to one frame a call).
+ * Utterance u's frames of this call are rows off[u] .. off[u]+T[u] of the
+ * fp32 logits [*, V]; T[u] <= 0: none.
+ *   width: beams kept per frame, 1 .. 128.  V: 2 .. 1024.  blank: 0 .. V-1.
+ *   state: device memory of w2v_ctc_beam_state_bytes(n_utt, V, width,
+ *      max_frames) bytes (-1: sizes out of range), 16-byte aligned.  max_frames bounds
+ *      an utterance's frames over all calls.  resume == 0 starts every
+ *      utterance anew (whatever state holds); resume != 0 continues from the
+ *      call before, with the same n_utt, V, blank, width and max_frames.
+ *      Calls on one state must be ordered.
+ *   Outputs, best first (none with n_best == 0; n_best <= width): n_ids[u][h]
+ *      tokens of hypothesis h (-1: fewer hypotheses than n_best), its first
+ *      min(n_ids, cap) tokens in ids[(u*n_best + h)*cap ..], the rest of its
+ *      cap entries -1; scores[u][h] its natural-log probability, fp64
+ *      (-inf: no hypothesis).
+ * Scores are held in 64 bits (the host decoder: 32).  Equal scores: a beam
+ * that stays before one that grows, then the better beam before the frame,
+ * then the smaller token.  A hypothesis less likely than 2^-1000 times the
+ * frame's best one is dropped.  A NaN logit is a token that cannot be
+ * emitted, as is -inf; a frame that can emit none leaves no hypothesis.  An
+ * utterance that would pass max_frames, or is continued from a state that was
+ * not started with these sizes, sets *err to 2, keeps its state and gives no
+ * hypothesis. */
+long long w2v_ctc_beam_state_bytes(int n_utt, int V, int width, int max_frames);
+int w2v_ctc_beam(const float* logits, const long long* off, const int* T, int n_utt, int V, int blank, int width,
+                 int max_frames, int resume, void* state, long long state_bytes, int n_best, int* ids,
+                 long long cap, int* n_ids, double* scores, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

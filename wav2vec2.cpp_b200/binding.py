@@ -80,6 +80,15 @@ SIGNATURES = {
     "w2v_pos_conv": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "w2v_attention": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _ll, _vp, _vp]),
     "w2v_ctc_greedy": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
+    "w2v_lora_workspace_bytes": (_ll, [_ll, _i, _i]),
+    "w2v_gemm_f16_lora": (_i, [_vp, _ll, _ll, _ll, _vp, _i, _vp, _ll, _vp, _vp, _ll, _i, _vp, _vp, _vp, _i, _i, _vp,
+                               _vp, _vp, _i, _vp, _ll, _vp, _vp]),
+    "w2v_gemm_q_lora": (_i, [_vp, _ll, _ll, _ll, _vp, _vp, _ll, _i, _i, _vp, _ll, _vp, _vp, _ll, _i, _vp, _vp, _vp,
+                             _i, _i, _vp, _vp, _vp, _i, _vp, _ll, _vp, _vp]),
+    "w2v_gemm_grouped_f16": (_i, [_vp, _ll, _ll, _ll, _vp, _i, _i, _vp, _ll, _vp, _vp, _ll, _i, _vp, _vp, _vp, _i,
+                                  _vp, _vp]),
+    "w2v_ctc_beam_state_bytes": (_ll, [_i, _i, _i, _i]),
+    "w2v_ctc_beam": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _ll, _i, _vp, _ll, _vp, _vp, _vp, _vp]),
 }
 
 _lib = None
@@ -359,3 +368,48 @@ class kernels:
     def ctc_greedy(logits, off, T, n_utt, V, ids, spans, n_spans, max_T, stream=0):
         kernels.check(lib().w2v_ctc_greedy(logits, off, T, n_utt, V, ids, spans, n_spans, max_T, stream or None),
                       "w2v_ctc_greedy")
+
+    @staticmethod
+    def lora_workspace_bytes(M, n_utt, rank):
+        n = lib().w2v_lora_workspace_bytes(M, n_utt, rank)
+        if n < 0:
+            raise EngineError("w2v_lora_workspace_bytes: sizes out of range")
+        return n
+
+    @staticmethod
+    def gemm_lora(A, lda, K, M, B, N, Cp, ldc, bias, resid, ldr, epilogue, lora_a, lora_b, lora_scale, n_adapters,
+                  rank, off, T, adapter, n_utt, workspace, workspace_bytes, err=0, stream=0):
+        kernels.check(lib().w2v_gemm_f16_lora(A, lda, K, M, B, N, Cp, ldc, bias or None, resid or None, ldr, epilogue,
+                                              lora_a, lora_b, lora_scale or None, n_adapters, rank, off, T, adapter,
+                                              n_utt, workspace, workspace_bytes, err or None, stream or None),
+                      "w2v_gemm_f16_lora")
+
+    @staticmethod
+    def gemm_q_lora(A, lda, K, M, Bq, Bs, ld_s, gguf_type, N, Cp, ldc, bias, resid, ldr, epilogue, lora_a, lora_b,
+                    lora_scale, n_adapters, rank, off, T, adapter, n_utt, workspace, workspace_bytes, err=0,
+                    stream=0):
+        kernels.check(lib().w2v_gemm_q_lora(A, lda, K, M, Bq, Bs, ld_s, gguf_type, N, Cp, ldc, bias or None,
+                                            resid or None, ldr, epilogue, lora_a, lora_b, lora_scale or None,
+                                            n_adapters, rank, off, T, adapter, n_utt, workspace, workspace_bytes,
+                                            err or None, stream or None), "w2v_gemm_q_lora")
+
+    @staticmethod
+    def gemm_grouped(A, lda, K, M, B, n_groups, N, Cp, ldc, bias, resid, ldr, epilogue, off, T, group, n_utt, err=0,
+                     stream=0):
+        kernels.check(lib().w2v_gemm_grouped_f16(A, lda, K, M, B, n_groups, N, Cp, ldc, bias or None, resid or None,
+                                                 ldr, epilogue, off, T, group, n_utt, err or None, stream or None),
+                      "w2v_gemm_grouped_f16")
+
+    @staticmethod
+    def ctc_beam_state_bytes(n_utt, V, width, max_frames):
+        n = lib().w2v_ctc_beam_state_bytes(n_utt, V, width, max_frames)
+        if n < 0:
+            raise EngineError("w2v_ctc_beam_state_bytes: sizes out of range")
+        return n
+
+    @staticmethod
+    def ctc_beam(logits, off, T, n_utt, V, blank, width, max_frames, resume, state, state_bytes, n_best, ids, cap,
+                 n_ids, scores, err=0, stream=0):
+        kernels.check(lib().w2v_ctc_beam(logits, off, T, n_utt, V, blank, width, max_frames, 1 if resume else 0,
+                                         state, state_bytes, n_best, ids or None, cap, n_ids or None, scores or None,
+                                         err or None, stream or None), "w2v_ctc_beam")
