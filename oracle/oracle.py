@@ -343,8 +343,50 @@ def ref_words_from_logits(ref: "RefOracle", logits):
     return text.value.decode(), [(w, float(times[2 * i]), float(times[2 * i + 1])) for i, w in enumerate(names)]
 
 
+def _table_beam_search(lg: np.ndarray, blank: int, beam: int) -> list[int]:
+    """The reference's prefix beam search (src/ops.h:151-251) restated on a
+    table of token tuples, fp32 log-probabilities with -1e30 for zero: for
+    hosts without the reference's build."""
+    f, floor = np.float32, np.float32(-1e30)
+
+    def lse(a, b):
+        if a <= f(-1e29):
+            return b
+        if b <= f(-1e29):
+            return a
+        hi, lo = (a, b) if a > b else (b, a)
+        return f(hi + np.log1p(np.exp(f(lo - hi))))
+
+    beams = {(): (f(0), floor)}
+    for row in lg:
+        lp = row - f(row.max() + np.log(np.exp(row - row.max()).sum(dtype=np.float32)))
+        new = {}
+
+        def put(prefix, i, value):
+            e = new.setdefault(prefix, [floor, floor])
+            e[i] = lse(e[i], value)
+
+        for prefix, (pb, pn) in beams.items():
+            total = lse(pb, pn)
+            put(prefix, 0, f(total + lp[blank]))
+            for c in range(len(row)):
+                if c == blank:
+                    continue
+                if prefix and c == prefix[-1]:
+                    put(prefix, 1, f(pn + lp[c]))
+                    put(prefix + (c,), 1, f(pb + lp[c]))
+                else:
+                    put(prefix + (c,), 1, f(total + lp[c]))
+        kept = sorted(new, key=lambda q: (-lse(*new[q]), q))[:beam]
+        beams = {q: tuple(new[q]) for q in kept}
+    best = min(beams, key=lambda q: (-lse(*beams[q]), q))
+    return list(best) if lse(*beams[best]) > floor else []
+
+
 def ref_beam_search(logits, blank: int, beam: int) -> list[int]:
     lg = np.ascontiguousarray(logits, np.float32)
+    if not ref_available():
+        return _table_beam_search(lg, blank, beam)
     T, V = lg.shape
     out = np.zeros(max(T, 1) + 1, np.int32)
     n = RefOracle.lib().w2vref_beam_search(_p(lg), T, V, blank, beam, _p(out), out.size)
