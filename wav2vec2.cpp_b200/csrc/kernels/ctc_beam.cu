@@ -471,7 +471,7 @@ extern "C" int w2v_ctc_beam(const float* logits, const long long* off, const int
     p.n_pairs = 0;
     for (int i = 0; i < width; i++) p.n_pairs += pairs_of(i, V, width);
     const int smem = (int)smem_layout(nullptr, nullptr, V, width, p.n_pairs);
-    if (smem > 48 * 1024 &&
+    if (smem > 40 * 1024 &&          // beside the static part
         cudaFuncSetAttribute(ctc_beam_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return W2V_ERR_LAUNCH;
     ctc_beam_kernel<<<n_utt, kThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);

@@ -1,28 +1,561 @@
-// Products whose weights depend on the row's utterance: low-rank adapters
-// beside a shared projection, and weight matrices per group of utterances.
+// Products whose weights depend on the row's utterance, on fp16 weights:
 //
 //   lora     y[r] = epi(W x[r] + bias + s_a B_a (A_a x[r])),  a = adapter of r's utterance
 //   grouped  y[r] = epi(W_g x[r] + bias_g),                   g = group of r's utterance
 //
-// 64 x 64 output tiles per block of 256 threads, operands through shared
-// memory as fp32, 4 x 4 outputs per thread on the FMA pipes.
-#include "common.cuh"
+// One persistent warp-specialised tcgen05 kernel serves both: TMA-fed 128-byte
+// swizzled operand tiles, fp32 accumulators in TMEM (two, so that the
+// epilogue of a tile overlaps the products of the next), single CTAs on
+// 128-row tiles or CTA pairs (cta_group::2) on 256-row tiles.  The tile width
+// is a launch parameter (any multiple of 32 up to 256: the MMA's N, the
+// weight box and the number of stages follow from it), so that narrow
+// outputs such as a head of 200 tokens do not pay for 256 columns.
+//
+// lora: tiles cover the packed rows as those of w2v_gemm_f16 do.  The adapters
+// are further K-blocks of the same accumulation: the first product (s_a A_a x,
+// lora_shrink.cu) lies in blocks of a tile's rows, one per adapter among them and
+// zero in the other rows, and is multiplied by that adapter's B.  The delta
+// thus costs rank / K of the main product per adapter in the tile, is added
+// in fp32 before the only rounding, and needs no pass of its own over y.  The
+// kernel starts while the first product runs and waits for it only when a
+// tile's main K-blocks have been issued.
+//
+// grouped: tiles are cut utterance by utterance (a warp-wide walk over the
+// utterances' lengths finds each tile, in order, so nothing is planned on the
+// host and no workspace is needed); rows past the utterance are computed and
+// not stored.
+#include <algorithm>
+
+#include "segments.cuh"
 #include "w2v_kernels.h"
 
 namespace w2v {
 namespace sg {
 
-constexpr int kTile = 64, kStep = 16;
-enum : int { kF16 = 0, kQ8 = 1, kQ4 = 2 };
+constexpr int kBM = 128, kBK = 64;
+constexpr int kNE = 8;                         // epilogue warps
+constexpr int kThreads = 64 + 32 * kNE;
+constexpr int kSmemCap = 232448;
+constexpr int kABytes = kBM * kBK * 2;
+constexpr int kEpiBytes = kNE * 4096;          // per warp: a 32 x 32 fp32 chunk, or two fp16 store boxes
+constexpr int kMaxStages = 8;
 
 struct Params {
-    const __half* A;
-    long long lda;
-    int K, N;
-    long long M;
-    const void* W;
-    const __half* scales;
-    long long ld_s;
+    int M, N, k_blocks;
+    int bn, n_tiles, m_tiles;                  // m_tiles: lora
+    int stages, b_bytes;
+    int vec, tma_c, bias_vec, bias_stride;     // wide stores; fp16 tile stores; wide bias loads; grouped: N
+    void* C;
+    long long ldc;
+    const float* bias;
+    const float* resid;
+    long long ldr;
+    int* err;
+    // lora
+    LoraPlan plan;
+    int lora;                                  // the plan holds adapters
+    // grouped
+    const long long* off;
+    const int* T;
+    const int* group;
+    int n_utt, n_groups;
+};
+
+// A tile's rows and weights.
+struct Tile {
+    int row0, end;                             // first row, one past the last valid row
+    int ni, group;
+};
+
+// Walks the utterances in steps of 32 (warp-collective): row tile m of the
+// batch, for m in ascending order.
+struct Walker {
+    int base = -32, before = 0;                // utterances base .. base + 31 (one per lane); row tiles before them
+    int first = 0, end = 0, group = 0, incl = 0, total = 0;
+
+    W2V_DEV void load(const Params& p, int tile_rows) {
+        const int u = base + (int)(threadIdx.x & 31);
+        int tiles = 0;
+        if (u < p.n_utt) {
+            const long long o = p.off[u];
+            const int t = p.T[u];
+            group = p.group[u];
+            if (o >= 0 && o < p.M && t > 0 && group >= 0 && group < p.n_groups) {
+                first = (int)o;
+                end = (int)min((long long)p.M, o + t);
+                tiles = (end - first + tile_rows - 1) / tile_rows;
+            }
+        }
+        incl = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, d);
+            if ((int)(threadIdx.x & 31) >= d) incl += v;
+        }
+        total = __shfl_sync(0xffffffffu, incl, 31);
+    }
+    // all row tiles of the batch
+    W2V_DEV int count(const Params& p, int tile_rows) {
+        int n = 0;
+        for (base = 0; base < p.n_utt; base += 32) {
+            load(p, tile_rows);
+            n += total;
+        }
+        base = -32;
+        total = 0;
+        return n;
+    }
+    // m < count(), not below an earlier call's
+    W2V_DEV void find(const Params& p, int tile_rows, int m, Tile& t) {
+        while (m >= before + total) {
+            before += total;
+            base += 32;
+            load(p, tile_rows);
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + incl > m);
+        const int src = __ffs(past) - 1;
+        const int prev = __shfl_sync(0xffffffffu, incl, src > 0 ? src - 1 : 0);
+        const int k = m - before - (src > 0 ? prev : 0);
+        t.row0 = __shfl_sync(0xffffffffu, first, src) + k * tile_rows;
+        t.end = __shfl_sync(0xffffffffu, end, src);
+        t.group = __shfl_sync(0xffffffffu, group, src);
+    }
+};
+
+W2V_DEV float epi_value(int epi, float x) { return epi == W2V_EPI_F16_GELU ? gelu_tanh(x) : x; }
+
+// The residual of this thread's 8 cells (4 columns) of a 32 x 32 chunk.
+W2V_DEV void load_resid(const Params& p, int row0, int end, int col0, float4 (&res)[8]) {
+    const int lane = threadIdx.x & 31, col = col0 + 4 * (lane & 7);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = row0 + (lane >> 3) + 4 * i;
+        res[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r >= end || col >= p.N) continue;
+        const float* src = p.resid + (long long)r * p.ldr + col;
+        if (p.vec && col + 3 < p.N) res[i] = *reinterpret_cast<const float4*>(src);
+        else {
+            res[i].x = src[0];
+            if (col + 1 < p.N) res[i].y = src[1];
+            if (col + 2 < p.N) res[i].z = src[2];
+            if (col + 3 < p.N) res[i].w = src[3];
+        }
+    }
+}
+
+// A staged 32 x 32 fp32 chunk to C: 8 threads per row, 4 columns each.
+template <int EPI>
+W2V_DEV void store_chunk(const Params& p, const float* stg, const float* bias, int row0, int end, int col0,
+                         const float4 (&res)[8]) {
+    const int lane = threadIdx.x & 31, cg = lane & 7, rs = lane >> 3;
+    const int col = col0 + 4 * cg;
+    if (col >= p.N) return;
+    const int n = min(4, p.N - col);
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (bias) {
+        if (p.bias_vec && n == 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(bias + col));
+            b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
+        } else {
+            for (int j = 0; j < n; j++) b[j] = __ldg(bias + col + j);
+        }
+    }
+    float4 xs[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) xs[i] = stage_get(stg, rs + 4 * i, cg);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = row0 + rs + 4 * i;
+        if (r >= end) continue;
+        float x[4] = {xs[i].x + b[0], xs[i].y + b[1], xs[i].z + b[2], xs[i].w + b[3]};
+        if (EPI == W2V_EPI_F32_RESID) { x[0] += res[i].x; x[1] += res[i].y; x[2] += res[i].z; x[3] += res[i].w; }
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = epi_value(EPI, x[j]);
+        const long long at = (long long)r * p.ldc + col;
+        if (EPI == W2V_EPI_F16 || EPI == W2V_EPI_F16_GELU) {
+            __half* c = reinterpret_cast<__half*>(p.C) + at;
+            if (p.vec && n == 4) *reinterpret_cast<uint2*>(c) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+            else
+                for (int j = 0; j < n; j++) c[j] = __float2half_rn(x[j]);
+        } else {
+            float* c = reinterpret_cast<float*>(p.C) + at;
+            if (p.vec && n == 4) *reinterpret_cast<float4*>(c) = make_float4(x[0], x[1], x[2], x[3]);
+            else
+                for (int j = 0; j < n; j++) c[j] = x[j];
+        }
+    }
+}
+
+// One row per lane of an fp16 chunk into a 32-row box of 64-byte rows (64-byte
+// swizzle) and out by one TMA tile store, which clips columns past N.
+template <int EPI>
+W2V_DEV void store_box(const Params& p, const CUtensorMap* tmC, float (&v)[32], const float* bias, uint8_t* box, int row0,
+                       int col0) {
+    const int lane = threadIdx.x & 31;
+    if (bias) {
+        if (p.bias_vec && col0 + 32 <= p.N) {
+            const float4* b4 = reinterpret_cast<const float4*>(bias + col0);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float4 b = __ldg(b4 + j);
+                v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) if (col0 + j < p.N) v[j] += __ldg(bias + col0 + j);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = epi_value(EPI, v[j]);
+    if (lane == 0) bulk_wait_group_read<1>();      // the store two boxes ago has read this one
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint4 u;
+        u.x = pack_half2(v[8 * j + 0], v[8 * j + 1]);
+        u.y = pack_half2(v[8 * j + 2], v[8 * j + 3]);
+        u.z = pack_half2(v[8 * j + 4], v[8 * j + 5]);
+        u.w = pack_half2(v[8 * j + 6], v[8 * j + 7]);
+        *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = u;
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_3d(tmC, box, col0, row0, 0);
+        bulk_commit_group();
+    }
+}
+
+template <int EPI, bool PAIR, bool LORA>
+__global__ void __launch_bounds__(kThreads, 1)
+seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmT,
+                const __grid_constant__ CUtensorMap tmL, const __grid_constant__ Params p) {
+    constexpr int CT = PAIR ? 2 : 1, kTileRows = kBM * CT;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    // identical offset in both CTAs of a pair: the MMA addresses the peer's operands at the leader's offsets
+    uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+    const int S = p.stages, stage_bytes = kABytes + p.b_bytes;
+    uint8_t* epi = smem + S * stage_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(epi + kEpiBytes);
+    uint64_t* empty = full + kMaxStages;
+    uint64_t* tfull = empty + kMaxStages;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* done = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+    const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+    const int n_units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], kNE * CT); }
+        mbar_init(done, 1);
+        fence_mbar_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+    }
+    if (warp == 1) {
+        if (PAIR) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+        else { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+    }
+    tc_fence_before();
+    if (PAIR) cluster_sync_all(); else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    Walker walk;
+    const int total = (LORA ? p.m_tiles : walk.count(p, kTileRows)) * p.n_tiles;
+    auto tile_at = [&](int tile) {
+        Tile t;
+        t.ni = tile % p.n_tiles;
+        const int m = tile / p.n_tiles;
+        if constexpr (LORA) { t.row0 = m * kTileRows; t.end = p.M; t.group = 0; }
+        else walk.find(p, kTileRows, m, t);
+        return t;
+    };
+    // further K-blocks of a row tile: adapters x parts x steps of 64 ranks
+    const int chunks = LORA ? (p.plan.rank + kBK - 1) / kBK : 0;
+
+    if (warp == 0) {
+        const uint32_t full_lead = PAIR ? mapa_shared(smem_u32(full), 0) : 0u;
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last_par = 0;
+        bool ok = true, waited = !LORA;
+        for (int tile = unit; tile < total && ok; tile += n_units) {
+            const Tile t = tile_at(tile);
+            if (lane == 0) {
+                auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int ka, int ra, int kb, int rb, int gb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
+                    uint8_t* sa = smem + stage * stage_bytes;
+                    if constexpr (PAIR) {
+                        const uint32_t fb = full_lead + (uint32_t)(stage * 8);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * stage_bytes);
+                        tma_load_2d_pair(sa, ma, fb, ka, ra + (int)rank * kBM);
+                        tma_load_4d_pair(sa + kABytes, mb, fb, kb, rb + (int)rank * (p.bn / 2), gb, 0);
+                    } else {
+                        mbar_arrive_expect_tx(&full[stage], stage_bytes);
+                        tma_load_2d(sa, ma, &full[stage], ka, ra);
+                        tma_load_4d(sa + kABytes, mb, &full[stage], kb, rb, gb, 0);
+                    }
+                    issued |= 1u << stage;
+                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                    if (++stage == S) { stage = 0; phase ^= 1u; }
+                };
+                for (int kb = 0; kb < p.k_blocks && ok; kb++)
+                    stage_in(&tmA, &tmB, kb * kBK, t.row0, kb * kBK, t.ni * p.bn, t.group);
+                if (LORA && p.lora) {
+                    if (!waited) { grid_dependency_wait(); waited = true; }
+                    const LoraTile lt = p.plan.tiles[t.row0 / kTileRows];
+                    for (int b = 0; b < lt.count && ok; b++) {
+                        const int ad = p.plan.adapter[lt.first + b];
+                        for (int part = 0; part < p.plan.parts; part++)
+                            for (int c = 0; c < chunks && ok; c++)
+                                stage_in(&tmT, &tmL, c * kBK,
+                                         (int)((part * p.plan.blocks + lt.first + b) * kTileRows), c * kBK,
+                                         t.ni * p.bn, ad);
+                    }
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        }
+        // no bulk copy may still be writing shared memory when the CTA (or its peer) exits
+        if (lane == 0 && rank == 0)
+            for (int s = 0; s < S; s++)
+                if (issued & (1u << s)) mbar_wait(&full[s], (last_par >> s) & 1u, p.err);
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = umma_idesc_f16(kTileRows, p.bn);
+            const uint32_t empty_peer = PAIR ? mapa_shared(smem_u32(empty), 1) : 0u;
+            const uint32_t tfull_peer = PAIR ? mapa_shared(smem_u32(tfull), 1) : 0u;
+            int stage = 0, it = 0;
+            uint32_t phase = 0;
+            bool ok = true, waited = !LORA;
+            for (int tile = unit; tile < total && ok; tile += n_units, it++) {
+                const int ab = it & 1;
+                if (!mbar_wait(&tempty[ab], ((uint32_t)(it >> 1) & 1u) ^ 1u, p.err)) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + (uint32_t)(ab * 256);
+                auto stage_mma = [&](bool first, int steps) {
+                    if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; return; }
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + kABytes;
+                    for (int kk = 0; kk < steps; kk++) {
+                        const uint64_t da = umma_desc_sw128(a0 + kk * 32), db = umma_desc_sw128(b0 + kk * 32);
+                        if constexpr (PAIR) umma_f16_pair(d, da, db, idesc, !(first && kk == 0));
+                        else umma_f16(d, da, db, idesc, !(first && kk == 0));
+                    }
+                    if constexpr (PAIR) {
+                        umma_commit_pair(smem_u32(&empty[stage]));
+                        umma_commit_pair(empty_peer + (uint32_t)(stage * 8));
+                    } else {
+                        umma_commit(&empty[stage]);
+                    }
+                    if (++stage == S) { stage = 0; phase ^= 1u; }
+                };
+                for (int kb = 0; kb < p.k_blocks && ok; kb++) stage_mma(kb == 0, kBK / 16);
+                if (LORA && p.lora && ok) {
+                    if (!waited) { grid_dependency_wait(); waited = true; }
+                    const int n = p.plan.tiles[tile / p.n_tiles].count * p.plan.parts;
+                    for (int b = 0; b < n; b++)
+                        for (int c = 0; c < chunks && ok; c++)
+                            stage_mma(false, min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16));
+                }
+                if (ok) {
+                    if constexpr (PAIR) {
+                        umma_commit_pair(smem_u32(&tfull[ab]));
+                        umma_commit_pair(tfull_peer + (uint32_t)(ab * 8));
+                    } else {
+                        umma_commit(&tfull[ab]);
+                    }
+                }
+            }
+            // no MMA may still be writing TMEM when it is freed (also after an expired wait)
+            if constexpr (PAIR) umma_commit_pair(smem_u32(done)); else umma_commit(done);
+            mbar_wait(done, 0, p.err);
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;                 // TMEM lane quarter this warp may access
+        const int n_ch = p.bn / 32, half = (n_ch + 1) / 2;
+        const int c0 = warp < 6 ? 0 : half, c1 = warp < 6 ? half : n_ch;   // two warps per quarter
+        const uint32_t tempty_lead = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0u;
+        float* stg = reinterpret_cast<float*>(epi + (warp - 2) * 4096);
+        constexpr bool kF16 = EPI == W2V_EPI_F16 || EPI == W2V_EPI_F16_GELU;
+        uint32_t nst = 0;
+        int it = 0;
+        for (int tile = unit; tile < total; tile += n_units, it++) {
+            const Tile t = tile_at(tile);
+            const int ab = it & 1;
+            const int row0 = t.row0 + (int)rank * kBM + q * 32;
+            const int col0 = t.ni * p.bn;
+            const float* bias = p.bias ? p.bias + (long long)t.group * p.bias_stride : nullptr;
+            // whole boxes inside the rows to be written (lora: the map clips at M)
+            const bool box = kF16 && p.tma_c && (LORA ? row0 < t.end : row0 + 32 <= t.end);
+            float4 res[8];
+            if (EPI == W2V_EPI_F32_RESID && c0 < c1) load_resid(p, row0, t.end, col0 + c0 * 32, res);
+            if (!mbar_wait(&tfull[ab], (uint32_t)(it >> 1) & 1u, p.err)) break;
+            tc_fence_after();
+            const uint32_t trow = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * 256);
+            if (kF16 && !box && nst) {          // boxes become the staging buffer
+                if (lane == 0) bulk_wait_group_read<0>();
+                __syncwarp();
+            }
+            if (row0 < t.end) {
+#pragma unroll 1
+                for (int c = c0; c < c1; c++) {
+                    const int cc = col0 + c * 32;
+                    if (cc >= p.N) break;
+                    float v[32];
+                    tmem_ld32(trow + (uint32_t)(c * 32), v);
+                    if (kF16 && box) {
+                        store_box<EPI>(p, &tmC, v, bias, reinterpret_cast<uint8_t*>(stg) + (nst & 1u) * 2048, row0, cc);
+                        nst++;
+                        continue;
+                    }
+                    float4 cur[8];
+                    if (EPI == W2V_EPI_F32_RESID) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) cur[i] = res[i];
+                        // the next chunk's residual is in flight while this chunk is stored
+                        if (c + 1 < c1) load_resid(p, row0, t.end, cc + 32, res);
+                    }
+                    __syncwarp();
+                    stage_put(stg, v);
+                    __syncwarp();
+                    store_chunk<EPI>(p, stg, bias, row0, t.end, cc, cur);
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_remote(tempty_lead + (uint32_t)(ab * 8));
+                else mbar_arrive(&tempty[ab]);
+            }
+        }
+        if (kF16) {      // the stores are complete before the CTA exits
+            if (lane == 0) bulk_wait_group<0>();
+            __syncwarp();
+        }
+    }
+
+    tc_fence_before();
+    if (PAIR) cluster_sync_all(); else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if (PAIR) tmem_dealloc_pair(tmem_base, 512); else tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// ── host side ───────────────────────────────────────────────────────────────
+
+static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        cudaDriverEntryPointQueryResult q;
+        void* f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// fp16 [.., rows, inner] with 64 x `box_rows` boxes, 128-byte swizzle.
+static int map_f16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, int box_rows) {
+    auto enc = get_encode();
+    if (!enc) return W2V_ERR_DRIVER;
+    const uint32_t box[4] = {kBK, (uint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims, strides, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? W2V_OK
+               : W2V_ERR_TENSOR_MAP;
+}
+
+struct Maps {
+    CUtensorMap a, b, c, t, l;
+};
+
+template <int EPI, bool PAIR, bool LORA>
+static int launch(const Maps& m, const Params& p, int tiles, bool dependent, cudaStream_t st) {
+    auto kern = seg_gemm_kernel<EPI, PAIR, LORA>;
+    static int max_units[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (PAIR) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = 2;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        n++;
+    }
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kSmemCap;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    if (!max_units[dev & 63]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap) != cudaSuccess)
+            return W2V_ERR_LAUNCH;
+        int sms = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2) return W2V_ERR_LAUNCH;
+        int units = sms / (PAIR ? 2 : 1);
+        if (PAIR) {          // pairs that can be resident at once (a GPC may leave an SM unpaired)
+            cfg.gridDim = dim3(2 * (sms / 2), 1, 1);
+            int c = 0;
+            if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess && c > 0) units = c;
+            cudaGetLastError();
+        }
+        max_units[dev & 63] = units;
+    }
+    const int units = tiles < max_units[dev & 63] ? tiles : max_units[dev & 63];
+    cfg.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)), 1, 1);
+    if (dependent) {         // start while the first product runs
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = ++n;
+    }
+    if (cudaLaunchKernelEx(&cfg, kern, m.a, m.b, m.c, m.t, m.l, p) != cudaSuccess) return W2V_ERR_LAUNCH;
+    return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
+}
+
+template <bool PAIR, bool LORA>
+static int launch_epi(int epi, const Maps& m, const Params& p, int tiles, bool dependent, cudaStream_t st) {
+    switch (epi) {
+        case W2V_EPI_F16: return launch<W2V_EPI_F16, PAIR, LORA>(m, p, tiles, dependent, st);
+        case W2V_EPI_F16_GELU: return launch<W2V_EPI_F16_GELU, PAIR, LORA>(m, p, tiles, dependent, st);
+        case W2V_EPI_F32: return launch<W2V_EPI_F32, PAIR, LORA>(m, p, tiles, dependent, st);
+        default: return launch<W2V_EPI_F32_RESID, PAIR, LORA>(m, p, tiles, dependent, st);
+    }
+}
+
+// Tile: width (a multiple of 32) and single CTAs or pairs, by waves x time per tile.
+static void pick_tile(int N, long long m_tiles1, long long m_tiles2, long long K, int* bn, bool* pair) {
+    double best = 1e300;
+    for (int pr = 0; pr < 2; pr++)
+        for (int w = 32; w <= 256; w += 32) {
+            if (w > 32 && w - 32 >= N) continue;
+            const long long tiles = (pr ? m_tiles2 : m_tiles1) * ((N + w - 1) / w);
+            const long long slots = pr ? 74 : 148;
+            const long long waves = (tiles + slots - 1) / slots;
+            const double cost = (double)waves * (w * (pr ? 1.0 : 1.1) + 48) * (K + 400);
+            if (cost < best) { best = cost; *bn = w; *pair = pr != 0; }
+        }
+}
+
+struct Call {
+    const void* A;
+    long long lda, K, M;
+    const void* B;
+    int n_mats, N;             // weight matrices (1: shared)
     void* C;
     long long ldc;
     const float* bias;
@@ -31,149 +564,62 @@ struct Params {
     int epilogue;
     const long long* off;
     const int* T;
-    const int* index;       // adapter or group of each utterance
-    int n_utt, n_index;
-    const __half* la;
-    const __half* lb;
-    const float* lscale;
-    int rank;
-    float* t;               // [M][rank] s_a A_a x
+    const int* index;
+    int n_utt;
+    int* err;
 };
 
-// The utterance that row r belongs to (off[u + 1] >= off[u] + T[u]), or -1.
-W2V_DEV int utterance_of(const long long* off, const int* T, int n_utt, long long r) {
-    int lo = 0, hi = n_utt;      // first utterance that ends after r
-    while (lo < hi) {
-        const int m = (lo + hi) / 2;
-        if (off[m] + max(T[m], 0) > r) hi = m; else lo = m + 1;
-    }
-    return lo < n_utt && off[lo] <= r ? lo : -1;
-}
-W2V_DEV int index_of(const Params& p, long long r) {
-    const int u = utterance_of(p.off, p.T, p.n_utt, r);
-    if (u < 0) return -1;
-    const int a = p.index[u];
-    return a >= 0 && a < p.n_index ? a : -1;
-}
-
-template <int WQ>
-W2V_DEV float weight(const Params& p, long long row, int n, int k) {
-    if (WQ == kF16) return __half2float(reinterpret_cast<const __half*>(p.W)[row * p.K + k]);
-    const __half d = p.scales[(k / 32) * p.ld_s + n];
-    int q;
-    if (WQ == kQ8) q = reinterpret_cast<const int8_t*>(p.W)[row * p.K + k];
-    else {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(p.W)[row * (p.K / 8) + k / 8];
-        const int j = k & 7;
-        q = (int)(w >> (4 * (j >> 1) + 16 * (j & 1)) & 15u) - 8;
-    }
-    return __half2float(__hmul(__int2half_rn(q), d));   // d * q rounded once
-}
-
-// t[r] = s_a A_a x[r]: one warp per row.
-__global__ void shrink_kernel(Params p) {
-    const long long r = blockIdx.x * 8LL + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (r >= p.M) return;
-    const int a = index_of(p, r);
-    const float s = a < 0 ? 0.f : p.lscale ? p.lscale[a] : 1.f;
-    for (int j = 0; j < p.rank; j++) {
-        float acc = 0.f;
-        if (a >= 0)
-            for (int k = lane; k < p.K; k += 32)
-                acc += __half2float(p.A[r * p.lda + k]) * __half2float(p.la[((long long)a * p.rank + j) * p.K + k]);
-        for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-        if (lane == 0) p.t[r * p.rank + j] = acc * s;
-    }
-}
-
-template <int WQ, bool GROUPED>
-__global__ void __launch_bounds__(256) tile_kernel(Params p) {
-    __shared__ float sx[kStep][kTile + 4], sw[kStep][kTile + 4];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int n0 = blockIdx.x * kTile;
-    long long r0 = blockIdx.y * (long long)kTile, r1 = p.M;
-    long long wrow = 0;
-    int g = 0;
-    if (GROUPED) {
-        const int u = blockIdx.z;
-        g = p.index[u];
-        if (g < 0 || g >= p.n_index) return;
-        r1 = min(p.M, p.off[u] + max(p.T[u], 0));
-        r0 += p.off[u];
-        wrow = (long long)g * p.N;
-    }
-    if (r0 >= r1) return;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += kStep) {
-        for (int i = tid; i < kTile * kStep; i += 256) {
-            const int k = i % kStep, m = i / kStep;
-            sx[k][m] = r0 + m < r1 ? __half2float(p.A[(r0 + m) * p.lda + k0 + k]) : 0.f;
-            sw[k][m] = n0 + m < p.N ? weight<WQ>(p, wrow + n0 + m, n0 + m, k0 + k) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kStep; k++) {
-            float x[4], w[4];
-            for (int i = 0; i < 4; i++) { x[i] = sx[k][ty * 4 + i]; w[i] = sw[k][tx * 4 + i]; }
-            for (int i = 0; i < 4; i++)
-                for (int j = 0; j < 4; j++) acc[i][j] += x[i] * w[j];
-        }
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; i++) {
-        const long long r = r0 + ty * 4 + i;
-        if (r >= r1) continue;
-        const int a = GROUPED ? -1 : index_of(p, r);
-        for (int j = 0; j < 4; j++) {
-            const int n = n0 + tx * 4 + j;
-            if (n >= p.N) continue;
-            float y = acc[i][j];
-            if (a >= 0) {
-                const __half* b = p.lb + ((long long)a * p.N + n) * p.rank;
-                for (int q = 0; q < p.rank; q++) y += p.t[r * p.rank + q] * __half2float(b[q]);
-            }
-            if (p.bias) y += p.bias[(long long)g * p.N + n];
-            if (p.epilogue == W2V_EPI_F16_GELU) y = gelu_tanh(y);
-            if (p.epilogue == W2V_EPI_F32_RESID) y += p.resid[r * p.ldr + n];
-            if (p.epilogue == W2V_EPI_F16 || p.epilogue == W2V_EPI_F16_GELU)
-                reinterpret_cast<__half*>(p.C)[r * p.ldc + n] = __float2half_rn(y);
-            else
-                reinterpret_cast<float*>(p.C)[r * p.ldc + n] = y;
-        }
-    }
-}
-
-static bool bad_common(const Params& p) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p.A), w = reinterpret_cast<uintptr_t>(p.W);
-    if (p.K <= 0 || p.K % 64 || p.M < 0 || p.M > 0x7fffffffLL || p.N <= 0 || p.lda < p.K || p.lda % 8 || p.ldc < p.N ||
-        ((a | w) & 15) || p.epilogue < W2V_EPI_F16 || p.epilogue > W2V_EPI_F32_RESID || p.n_utt < 0)
+static bool refused(const Call& c) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(c.A), b = reinterpret_cast<uintptr_t>(c.B);
+    if (c.K <= 0 || c.K % 64 || c.K > 0x7fffffffLL || c.M < 0 || c.M > 0x7fffffffLL - 512 || c.N <= 0 || c.lda < c.K ||
+        c.lda % 8 || c.ldc < c.N || ((a | b) & 15) || c.epilogue < W2V_EPI_F16 || c.epilogue > W2V_EPI_F32_RESID ||
+        c.n_utt < 0)
         return true;
-    return p.M > 0 && (!p.A || !p.W || !p.C || (p.epilogue == W2V_EPI_F32_RESID && (!p.resid || p.ldr < p.N)) ||
-                       (p.n_utt > 0 && (!p.off || !p.T || !p.index)));
+    return c.M > 0 && (!c.A || !c.B || !c.C || (c.epilogue == W2V_EPI_F32_RESID && (!c.resid || c.ldr < c.N)) ||
+                       (c.n_utt > 0 && (!c.off || !c.T || !c.index)));
 }
 
-static int lora(Params p, int wq, const void* lora_a, const void* lora_b, const float* lora_scale, int n_adapters,
-                int rank, void* workspace, long long workspace_bytes, cudaStream_t st) {
-    if (bad_common(p) || rank < 8 || rank > 128 || rank % 8 || n_adapters <= 0 || !lora_a || !lora_b ||
-        ((reinterpret_cast<uintptr_t>(lora_a) | reinterpret_cast<uintptr_t>(lora_b)) & 15))
-        return W2V_ERR_ARGS;
-    if (p.M == 0) return W2V_OK;
-    const long long need = w2v_lora_workspace_bytes(p.M, p.n_utt, rank);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 127)) return W2V_ERR_ARGS;
-    if (workspace_bytes < need) return W2V_ERR_CAPACITY;
-    p.la = reinterpret_cast<const __half*>(lora_a);
-    p.lb = reinterpret_cast<const __half*>(lora_b);
-    p.lscale = lora_scale;
-    p.n_index = n_adapters;
-    p.rank = rank;
-    p.t = reinterpret_cast<float*>(workspace);
-    shrink_kernel<<<(unsigned)((p.M + 7) / 8), 256, 0, st>>>(p);
-    const dim3 grid((p.N + kTile - 1) / kTile, (unsigned)((p.M + kTile - 1) / kTile));
-    if (wq == kF16) tile_kernel<kF16, false><<<grid, 256, 0, st>>>(p);
-    else if (wq == kQ8) tile_kernel<kQ8, false><<<grid, 256, 0, st>>>(p);
-    else tile_kernel<kQ4, false><<<grid, 256, 0, st>>>(p);
-    return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
+// Parameters and maps that both products share.
+static int common(const Call& c, int bn, bool pair, Params& p, Maps& m) {
+    const bool f16 = c.epilogue == W2V_EPI_F16 || c.epilogue == W2V_EPI_F16_GELU;
+    const uintptr_t C = reinterpret_cast<uintptr_t>(c.C), R = reinterpret_cast<uintptr_t>(c.resid);
+    p.M = (int)c.M;
+    p.N = c.N;
+    p.k_blocks = (int)(c.K / kBK);
+    p.bn = bn;
+    p.n_tiles = (c.N + bn - 1) / bn;
+    p.b_bytes = (pair ? bn / 2 : bn) * kBK * 2;
+    p.stages = std::min(kMaxStages, (kSmemCap - 1024 - 256 - kEpiBytes) / (kABytes + p.b_bytes));
+    p.vec = c.ldc % 4 == 0 && C % (f16 ? 8 : 16) == 0 &&
+            (c.epilogue != W2V_EPI_F32_RESID || (c.ldr % 4 == 0 && R % 16 == 0));
+    p.bias_vec = reinterpret_cast<uintptr_t>(c.bias) % 16 == 0 && (c.n_mats == 1 || c.N % 4 == 0);
+    p.bias_stride = c.n_mats == 1 ? 0 : c.N;
+    p.C = c.C;
+    p.ldc = c.ldc;
+    p.bias = c.bias;
+    p.resid = c.resid;
+    p.ldr = c.ldr;
+    p.err = c.err;
+    const uint64_t ad[2] = {(uint64_t)c.K, (uint64_t)c.M}, as[1] = {(uint64_t)c.lda * 2};
+    int rc = map_f16(&m.a, c.A, 2, ad, as, kBM);
+    if (rc) return rc;
+    const uint64_t bd[4] = {(uint64_t)c.K, (uint64_t)c.N, (uint64_t)c.n_mats, 1};
+    const uint64_t bs[3] = {(uint64_t)c.K * 2, (uint64_t)c.K * 2 * c.N, (uint64_t)c.K * 2 * c.N * c.n_mats};
+    rc = map_f16(&m.b, c.B, 4, bd, bs, pair ? bn / 2 : bn);
+    if (rc) return rc;
+    m.c = m.t = m.l = m.a;
+    // fp16 C by 32 x 32 boxes; a store clips the innermost dimension at 16-byte granularity only
+    p.tma_c = f16 && c.ldc % 8 == 0 && c.N % 8 == 0 && C % 16 == 0;
+    if (p.tma_c) {
+        const uint64_t cd[3] = {(uint64_t)c.N, (uint64_t)c.M, 1};
+        const uint64_t cs[2] = {(uint64_t)c.ldc * 2, (uint64_t)c.ldc * 2 * c.M};
+        const uint32_t cbox[3] = {32, 32, 1}, es[3] = {1, 1, 1};
+        if (get_encode()(&m.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, c.C, cd, cs, cbox, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return W2V_ERR_TENSOR_MAP;
+    }
+    return W2V_OK;
 }
 
 }  // namespace sg
@@ -183,7 +629,7 @@ using namespace w2v::sg;
 
 extern "C" long long w2v_lora_workspace_bytes(long long M, int n_utt, int rank) {
     if (M < 0 || n_utt < 0 || rank < 8 || rank > 128 || rank % 8) return -1;
-    return (M * rank * 4 + 127) / 128 * 128;
+    return lora_workspace(M, n_utt, rank);
 }
 
 extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long long M, const void* B, int N, void* C,
@@ -191,46 +637,80 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
                                  const void* lora_a, const void* lora_b, const float* lora_scale, int n_adapters,
                                  int rank, const long long* off, const int* T, const int* adapter, int n_utt,
                                  void* workspace, long long workspace_bytes, int* err, void* stream) {
-    if (K > 0x7fffffffLL) return W2V_ERR_ARGS;
-    Params p = {};
-    p.A = reinterpret_cast<const __half*>(A); p.lda = lda; p.K = (int)K; p.M = M; p.W = B; p.N = N; p.C = C;
-    p.ldc = ldc; p.bias = bias; p.resid = resid; p.ldr = ldr; p.epilogue = epilogue;
-    p.off = off; p.T = T; p.index = adapter; p.n_utt = n_utt;
-    return lora(p, kF16, lora_a, lora_b, lora_scale, n_adapters, rank, workspace, workspace_bytes,
-                reinterpret_cast<cudaStream_t>(stream));
-}
-
-extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long long M, const void* Bq, const void* Bs,
-                               long long ld_s, int gguf_type, int N, void* C, long long ldc, const float* bias,
-                               const float* resid, long long ldr, int epilogue, const void* lora_a,
-                               const void* lora_b, const float* lora_scale, int n_adapters, int rank,
-                               const long long* off, const int* T, const int* adapter, int n_utt, void* workspace,
-                               long long workspace_bytes, int* err, void* stream) {
-    const int wq = gguf_type == 8 ? kQ8 : gguf_type == 2 ? kQ4 : 0;
-    if (!wq || K > 0x7fffffffLL || !Bs || (reinterpret_cast<uintptr_t>(Bs) & 15) || ld_s < N || ld_s % 8)
+    const Call c{A, lda, K, M, B, 1, N, C, ldc, bias, resid, ldr, epilogue, off, T, adapter, n_utt, err};
+    if (refused(c) || !B || rank < 8 || rank > 128 || rank % 8 || n_adapters <= 0 || !lora_a || !lora_b ||
+        ((reinterpret_cast<uintptr_t>(lora_a) | reinterpret_cast<uintptr_t>(lora_b)) & 15))
         return W2V_ERR_ARGS;
+    if (M == 0) return W2V_OK;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 127)) return W2V_ERR_ARGS;
+    if (workspace_bytes < lora_workspace(M, n_utt, rank)) return W2V_ERR_CAPACITY;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     Params p = {};
-    p.A = reinterpret_cast<const __half*>(A); p.lda = lda; p.K = (int)K; p.M = M; p.W = Bq; p.N = N; p.C = C;
-    p.scales = reinterpret_cast<const __half*>(Bs); p.ld_s = ld_s;
-    p.ldc = ldc; p.bias = bias; p.resid = resid; p.ldr = ldr; p.epilogue = epilogue;
-    p.off = off; p.T = T; p.index = adapter; p.n_utt = n_utt;
-    return lora(p, wq, lora_a, lora_b, lora_scale, n_adapters, rank, workspace, workspace_bytes,
-                reinterpret_cast<cudaStream_t>(stream));
+    Maps m;
+    int bn = 256;
+    bool pair = false;
+    pick_tile(N, (M + 127) / 128, (M + 255) / 256, K, &bn, &pair);
+    int rc = common(c, bn, pair, p, m);
+    if (rc) return rc;
+    const int tile_rows = pair ? 256 : 128;
+    p.m_tiles = (int)((M + tile_rows - 1) / tile_rows);
+    p.lora = n_utt > 0;
+    p.plan = lora_plan(workspace, M, n_utt, rank, tile_rows, epilogue == W2V_EPI_F16 || epilogue == W2V_EPI_F16_GELU ? 1 : 2);
+    if (p.lora) {
+        if (p.plan.parts * p.plan.blocks * tile_rows > 0x7fffffffLL) return W2V_ERR_ARGS;
+        const uint64_t td[2] = {(uint64_t)rank, (uint64_t)(p.plan.parts * p.plan.blocks * tile_rows)};
+        const uint64_t ts[1] = {(uint64_t)rank * 2};
+        rc = map_f16(&m.t, p.plan.t, 2, td, ts, kBM);
+        if (rc) return rc;
+        const uint64_t ld[4] = {(uint64_t)rank, (uint64_t)N, (uint64_t)n_adapters, 1};
+        const uint64_t ls[3] = {(uint64_t)rank * 2, (uint64_t)rank * 2 * N, (uint64_t)rank * 2 * N * n_adapters};
+        rc = map_f16(&m.l, lora_b, 4, ld, ls, pair ? bn / 2 : bn);
+        if (rc) return rc;
+        LoraArgs a;
+        a.x = reinterpret_cast<const __half*>(A);
+        a.lda = lda;
+        a.K = (int)K;
+        a.M = M;
+        a.a = reinterpret_cast<const __half*>(lora_a);
+        a.scale = lora_scale;
+        a.n_adapters = n_adapters;
+        a.off = off;
+        a.T = T;
+        a.adapter = adapter;
+        a.n_utt = n_utt;
+        rc = lora_shrink(a, p.plan, st);
+        if (rc) return rc;
+    }
+    const long long tiles = (long long)p.m_tiles * p.n_tiles;
+    if (tiles > 0x7fffffffLL / 2) return W2V_ERR_ARGS;
+    return pair ? launch_epi<true, true>(epilogue, m, p, (int)tiles, p.lora, st)
+                : launch_epi<false, true>(epilogue, m, p, (int)tiles, p.lora, st);
 }
 
 extern "C" int w2v_gemm_grouped_f16(const void* A, long long lda, long long K, long long M, const void* B,
                                     int n_groups, int N, void* C, long long ldc, const float* bias,
                                     const float* resid, long long ldr, int epilogue, const long long* off,
                                     const int* T, const int* group, int n_utt, int* err, void* stream) {
-    if (K > 0x7fffffffLL || n_groups <= 0) return W2V_ERR_ARGS;
-    Params p = {};
-    p.A = reinterpret_cast<const __half*>(A); p.lda = lda; p.K = (int)K; p.M = M; p.W = B; p.N = N; p.C = C;
-    p.ldc = ldc; p.bias = bias; p.resid = resid; p.ldr = ldr; p.epilogue = epilogue;
-    p.off = off; p.T = T; p.index = group; p.n_index = n_groups; p.n_utt = n_utt;
-    if (bad_common(p)) return W2V_ERR_ARGS;
+    const Call c{A, lda, K, M, B, n_groups, N, C, ldc, bias, resid, ldr, epilogue, off, T, group, n_utt, err};
+    if (n_groups <= 0 || refused(c)) return W2V_ERR_ARGS;
     if (M == 0 || n_utt == 0) return W2V_OK;
-    if (n_utt > 65535) return W2V_ERR_CAPACITY;
-    const dim3 grid((N + kTile - 1) / kTile, (unsigned)((M + kTile - 1) / kTile), n_utt);
-    tile_kernel<kF16, true><<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-    return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
+    Params p = {};
+    Maps m;
+    int bn = 256;
+    bool pair = false;
+    // row tiles: at most one more than its rows need per utterance
+    const long long more = n_utt < M ? n_utt : M;
+    pick_tile(N, M / 128 + more, M / 256 + more, K, &bn, &pair);
+    int rc = common(c, bn, pair, p, m);
+    if (rc) return rc;
+    p.off = off;
+    p.T = T;
+    p.group = group;
+    p.n_utt = n_utt;
+    p.n_groups = n_groups;
+    const long long tiles = (M / (pair ? 256 : 128) + more) * p.n_tiles;
+    if (tiles > 0x7fffffffLL / 2) return W2V_ERR_ARGS;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return pair ? launch_epi<true, false>(epilogue, m, p, (int)tiles, false, st)
+                : launch_epi<false, false>(epilogue, m, p, (int)tiles, false, st);
 }
