@@ -43,7 +43,6 @@ namespace cb {
 
 constexpr int kMaxWidth = 128;
 constexpr int kMaxVocab = 1024;
-constexpr int kThreads = 256;
 
 typedef unsigned long long u64;
 
@@ -60,12 +59,12 @@ struct Header {
     double log_z;        // sum of the logarithms of the rows' sums
 };
 
-struct Beams {           // structure of arrays, `width` long each
-    double *pb, *pn;
-    u64* mask;
-    int *node, *last, *len, *pnode, *par, *head;
+// One beam, as the state keeps it between calls.
+struct SavedBeam {
+    double pb, pn;
+    u64 mask;
+    int node, last, len, pnode, par, head;
 };
-constexpr int kBeamBytes = 3 * 8 + 6 * 4;
 
 struct Layout {
     long long beams, nodes, masks, bytes;
@@ -74,25 +73,11 @@ __host__ __device__ inline Layout layout(int width, long long max_frames) {
     Layout l;
     const long long n = (long long)width * max_frames + 1;
     l.beams = sizeof(Header);
-    l.nodes = (l.beams + (long long)width * kBeamBytes + 15) / 16 * 16;
+    l.nodes = (l.beams + (long long)width * (long long)sizeof(SavedBeam) + 15) / 16 * 16;
     l.masks = l.nodes + n * (long long)sizeof(Node);
     l.bytes = (l.masks + n * 8 + 255) / 256 * 256;
     return l;
 }
-__host__ __device__ inline Beams beams_at(void* base, int width) {
-    Beams b;
-    b.pb = reinterpret_cast<double*>(base);
-    b.pn = b.pb + width;
-    b.mask = reinterpret_cast<u64*>(b.pn + width);
-    b.node = reinterpret_cast<int*>(b.mask + width);
-    b.last = b.node + width;
-    b.len = b.last + width;
-    b.pnode = b.len + width;
-    b.par = b.pnode + width;
-    b.head = b.par + width;
-    return b;
-}
-
 __host__ __device__ inline u64 tag_of(int V, int blank, int width, int max_frames) {
     return 0x6265616d00000000ull ^ (u64)V << 52 ^ (u64)blank << 40 ^ (u64)width << 32 ^ (u64)max_frames;
 }
@@ -109,6 +94,7 @@ struct Params {
     double* scores;
     int* err;
     int n_pairs;         // extension candidates (i, j): (i + 1) j <= width
+    int slots;           // rows in the ring
 };
 
 // Tokens of rank 0 .. n_tok - 1 can extend a beam.
@@ -118,76 +104,148 @@ __host__ __device__ inline int pairs_of(int i, int V, int width) {
     return n < V - 1 ? n : V - 1;
 }
 
-struct Smem {
-    double* p;           // [V] exp(logit - max)
-    double* sp;          // [n_tok] the same by rank
-    u64* key;            // [width + n_pairs]
-    uint32_t* order;     // [width + n_pairs] order among equal values: stays, then (beam, token)
-    uint32_t* bits;      // [width][words] tokens whose extension of the beam is a beam
-    int* stok;           // [n_tok] token by rank
-    int* sel;            // [width] candidate of each new beam
-    int* slot;           // [width] new place of an old beam, -1: dropped
-    int* back;           // [width] new beams whose node was found again
-    uint16_t* pair;      // [n_pairs] beam in the high byte, rank in the low
-    Beams b[2];
-    int words;
+// A frame's row as the search needs it: by_rank[n_tok], p[V], log_z.
+struct Ranked {
+    double p;            // exp(logit - max), largest first (equal ones by token)
+    int tok, pad;
 };
-__host__ __device__ inline long long smem_layout(Smem* s, uint8_t* base, int V, int width, int n_pairs) {
-    const int nt = n_tokens(V, width), nc = width + n_pairs, words = (V + 31) / 32;
-    long long o = 0;
-    auto take = [&](long long bytes) { const long long at = o; o += (bytes + 15) / 16 * 16; return base + at; };
-    uint8_t* p = take(8LL * V);
-    uint8_t* sp = take(8LL * nt);
-    uint8_t* key = take(8LL * nc);
-    uint8_t* b0 = take((long long)width * kBeamBytes);
-    uint8_t* b1 = take((long long)width * kBeamBytes);
-    uint8_t* order = take(4LL * nc);
-    uint8_t* bits = take(4LL * width * words);
-    uint8_t* stok = take(4LL * nt);
-    uint8_t* sel = take(4LL * width);
-    uint8_t* slot = take(4LL * width);
-    uint8_t* back = take(4LL * width);
-    uint8_t* pair = take(2LL * n_pairs);
-    if (s) {
-        s->p = reinterpret_cast<double*>(p);
-        s->sp = reinterpret_cast<double*>(sp);
-        s->key = reinterpret_cast<u64*>(key);
-        s->b[0] = beams_at(b0, width);
-        s->b[1] = beams_at(b1, width);
-        s->order = reinterpret_cast<uint32_t*>(order);
-        s->bits = reinterpret_cast<uint32_t*>(bits);
-        s->stok = reinterpret_cast<int*>(stok);
-        s->sel = reinterpret_cast<int*>(sel);
-        s->slot = reinterpret_cast<int*>(slot);
-        s->back = reinterpret_cast<int*>(back);
-        s->pair = reinterpret_cast<uint16_t*>(pair);
-        s->words = words;
-    }
-    return o;
+struct Row {
+    Ranked* by_rank;
+    double* p;           // by token
+    double* log_z;       // logarithm of the sum of p (0: nothing can be emitted)
+};
+__host__ __device__ inline int row_bytes(int V, int width) { return (n_tokens(V, width) * 16 + (V + 1) * 8 + 15) / 16 * 16; }
+W2V_DEV Row row_at(uint8_t* base, int V, int n_tok) {
+    Row r;
+    r.by_rank = reinterpret_cast<Ranked*>(base);
+    r.p = reinterpret_cast<double*>(base + n_tok * 16);
+    r.log_z = r.p + V;
+    return r;
 }
+
+// A candidate: its beam and, for an extension, its token + 1 (0: the stay).
+W2V_DEV uint32_t pack_cand(int beam, int tok) { return (uint32_t)beam | (uint32_t)(tok + 1) << 8; }
+W2V_DEV int beam_of(uint32_t c) { return (int)(c & 255u); }
+W2V_DEV int token_of(uint32_t c) { return (int)(c >> 8) - 1; }
+
+// The beams of a frame, one 16-byte word of each beam per array.
+template <int MW>
+struct Beams {
+    struct Prob { double pb, total; } prob[MW];
+    struct Info { int node, last, len, pnode; } info[MW];
+    struct Link { uint32_t mask[2]; int head, par; } link[MW];   // mask: tokens (mod 64) the node was ever extended by
+    double pn[MW];
+};
+// Candidates of a frame at most: MW stays and the sum of MW / i + 1 for i = 1 .. MW pairs, rounded up.
+__host__ __device__ constexpr int max_live(int MW) {
+    int n = MW;
+    for (int i = 1; i <= MW; i++) n += MW / i + 1;
+    return (n + 31) / 32 * 32;
+}
+
+template <int MW>
+struct Shared {
+    uint32_t key32[max_live(MW)];    // leading bits of the values of the candidates in the running
+    u64 key[max_live(MW)];           // the values
+    Beams<MW> beams[2];
+    struct Stay { double b, n; } stay[MW];       // the stays' pb', pn'
+    struct Sel { u64 key; uint32_t cand, pad; } sel[MW];   // the new beams in order
+    uint32_t cand[max_live(MW)];     // which candidates they are
+    int slot[MW];                    // new place of an old beam that stays, -1: dropped
+    int back[MW];                    // new beams whose node was found again
+    int pair_at[MW];
+    uint16_t pair[max_live(MW) - MW];    // beam in the high byte, rank in the low
+    int n_live, n_back, expired;
+    int place_sum;                   // of the candidates: less than all different ones add up to where values are equal
+    uint32_t least_hi[8];
+    // of the last frame, for the hypotheses
+    int nb, cur;
+    long long exp2;
+    double log_z;
+};
 
 // A logit as the search sees it: NaN cannot be emitted, +inf is the largest number.
 W2V_DEV float clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
+W2V_DEV u64 bits_of(double x) { return (u64)__double_as_longlong(x); }   // positive numbers order as their bits
+W2V_DEV double value_of(u64 k) { return __longlong_as_double((long long)k); }
 
-__global__ void __launch_bounds__(kThreads) ctc_beam_kernel(Params p) {
+// Row producer: one warp turns the logits of a frame into a Row.
+W2V_DEV void make_row(const float* x, int V, int blank, int n_tok, float mx, const Row& r) {
+    const int lane = threadIdx.x & 31;
+    double z = 0.0;
+    for (int v = lane; v < V; v += 32) {
+        const float l = clean(x[v]);
+        const double e = l == -INFINITY ? 0.0 : exp((double)l - (double)mx);
+        r.p[v] = e;
+        z += e;
+    }
+    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    __syncwarp();
+    for (int v = lane; v < V; v += 32) {
+        const u64 e = bits_of(r.p[v]);
+        int rank = 0;
+        for (int w = 0; w < V; w++) {
+            const u64 f = bits_of(r.p[w]);
+            rank += w != blank && (w < v ? f >= e : f > e);
+        }
+        if (v != blank && rank < n_tok) r.by_rank[rank] = Ranked{value_of(e), v, 0};
+    }
+    if (lane == 0) *r.log_z = z > 0.0 ? log(z) : 0.0;
+    __syncwarp();
+}
+
+// The best candidate of a frame is at least half and less than four times the
+// best beam, which is held between 1 and 2: what is to be kept lies between
+// 2^-1001 and 8.  Counted from 2^-1003, the exponent of such a value takes 10 bits,
+// which leaves 22 of the fraction for a 32-bit key.
+constexpr u64 kLeast = (u64)20 << 52;
+W2V_DEV uint32_t leading(u64 k) { return (uint32_t)((k - kLeast) >> 30); }
+
+// Barrier of the NC search warps.
+template <int NC>
+W2V_DEV void search_sync() {
+    if (NC == 1) __syncwarp();
+    else asm volatile("barrier.sync 1, %0;" ::"n"(NC * 32) : "memory");
+}
+// How many of the keys are larger than k: 32 of every `step`, as long as they
+// begin before n (keys behind the last are 0).
+W2V_DEV int count_above(const uint32_t* keys, int n, int step, uint32_t k) {
+    int c0 = 0, c1 = 0;
+    for (int d = 0; d < n; d += step) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = reinterpret_cast<const uint4*>(keys + d)[i];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            c0 += (v[i].x > k) + (v[i].y > k);
+            c1 += (v[i].z > k) + (v[i].w > k);
+        }
+    }
+    return c0 + c1;
+}
+
+// NC search warps (the chain from frame to frame; beam i is thread i's) and
+// NP row producers (frame t: warp t % NP), a ring of rows between them.
+template <int NC, int NP, int MW>
+__global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
+    constexpr int NT = NC * 32;
+    constexpr int kPairs = (max_live(MW) - MW + NT - 1) / NT;       // of a thread
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ float red_f[kThreads / 32];
-    __shared__ double red_d[kThreads / 32];
-    __shared__ u64 best_key;
-    __shared__ int n_new, n_back;
-    Smem s;
-    smem_layout(&s, smem_raw, p.V, p.width, p.n_pairs);
+    __shared__ uint64_t full[2 * NP], empty[2 * NP];
+    Shared<MW>& s = *reinterpret_cast<Shared<MW>*>(smem_raw);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(smem_raw + sizeof(Shared<MW>));   // [width][words]
     const int u = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int W = p.width, V = p.V, nt = n_tokens(V, W);
+    const int W = p.width, V = p.V, n_tok = n_tokens(V, W), words = (V + 31) / 32;
+    uint8_t* rows = smem_raw + sizeof(Shared<MW>) + (W * words * 4 + 15) / 16 * 16;
     const Layout lay = layout(W, p.max_frames);
     uint8_t* st = p.state + (long long)u * lay.bytes;
     Header* hdr = reinterpret_cast<Header*>(st);
-    Beams saved = beams_at(st + lay.beams, W);
+    SavedBeam* saved = reinterpret_cast<SavedBeam*>(st + lay.beams);
     Node* nodes = reinterpret_cast<Node*>(st + lay.nodes);
     u64* masks = reinterpret_cast<u64*>(st + lay.masks);
 
-    int T = p.T[u] > 0 ? p.T[u] : 0;
-    int frames = 0, nb = 1, cur = 0;
+    const int T = p.T[u] > 0 ? p.T[u] : 0;
+    int frames = 0, nb = 1;
     long long exp2 = 0;
     double log_z = 0.0;
     const u64 tag = tag_of(V, p.blank, W, p.max_frames);
@@ -200,235 +258,387 @@ __global__ void __launch_bounds__(kThreads) ctc_beam_kernel(Params p) {
     }
     refused = refused || T > p.max_frames - frames;
     if (refused && tid == 0) report_error(p.err, kErrBadArgs);
-    Beams b = s.b[0];
-    if (tid < W && tid < nb && !refused) {
-        if (p.resume) {
-            b.pb[tid] = saved.pb[tid];
-            b.pn[tid] = saved.pn[tid];
-            b.mask[tid] = saved.mask[tid];
-            b.node[tid] = saved.node[tid];
-            b.last[tid] = saved.last[tid];
-            b.len[tid] = saved.len[tid];
-            b.pnode[tid] = saved.pnode[tid];
-            b.par[tid] = saved.par[tid];
-            b.head[tid] = saved.head[tid];
-        } else {
-            b.pb[0] = 1.0;
-            b.pn[0] = 0.0;
-            b.mask[0] = 0;
-            b.node[0] = 0;
-            b.last[0] = -1;
-            b.len[0] = 0;
-            b.pnode[0] = -1;
-            b.par[0] = -1;
-            b.head[0] = -1;
-            nodes[0] = Node{-1, -1, -1, -1};
+    for (int i = tid; i < W * words; i += (NC + NP) * 32) bits[i] = 0;
+    for (int i = tid; i < max_live(MW); i += (NC + NP) * 32) s.key32[i] = 0;
+    if (tid < 2 * NP) {
+        mbar_init(&full[tid], 1);
+        mbar_init(&empty[tid], 1);
+    }
+    if (tid == 0) {
+        fence_mbar_init();
+        s.n_live = 0;
+        s.n_back = 0;
+        s.expired = 0;
+        s.place_sum = 0;
+    }
+    if (warp == 0) {         // where each beam's pairs start
+        int before = 0;
+        for (int i0 = 0; i0 < W; i0 += 32) {
+            const int n = i0 + lane < W ? pairs_of(i0 + lane, V, W) : 0;
+            int incl = n;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += v;
+            }
+            if (i0 + lane < W) s.pair_at[i0 + lane] = before + incl - n;
+            before += __shfl_sync(0xffffffffu, incl, 31);
         }
     }
-    for (int i = tid; i < W * s.words; i += kThreads) s.bits[i] = 0;
-    if (tid < W) {
-        int at = 0;
-        for (int i = 0; i < tid; i++) at += pairs_of(i, V, W);
-        for (int j = 0; j < pairs_of(tid, V, W); j++) s.pair[at + j] = (uint16_t)(tid << 8 | j);
+    __syncthreads();
+    for (int i = warp; i < W; i += NC + NP)
+        for (int k = lane; k < pairs_of(i, V, W); k += 32) s.pair[s.pair_at[i] + k] = (uint16_t)(i << 8 | k);
+    double my_pb = 0.0, my_pn = 0.0, my_total = 0.0;     // this thread's beam
+    int my_last = -1, my_par = -1;
+    if (tid < nb && !refused) {
+        SavedBeam v{1.0, 0.0, 0, 0, -1, 0, -1, -1, -1};
+        if (p.resume) v = saved[tid];
+        else nodes[0] = Node{-1, -1, -1, -1};
+        my_pb = v.pb;
+        my_pn = v.pn;
+        my_total = my_pb + my_pn;
+        my_last = v.last;
+        my_par = v.par;
+        s.beams[0].prob[tid] = {my_pb, my_total};
+        s.beams[0].pn[tid] = my_pn;
+        s.beams[0].info[tid] = {v.node, v.last, v.len, v.pnode};
+        s.beams[0].link[tid] = {{(uint32_t)v.mask, (uint32_t)(v.mask >> 32)}, v.head, v.par};
+        if (my_par >= 0) atomicOr(&bits[my_par * words + (my_last >> 5)], 1u << (my_last & 31));
     }
     __syncthreads();
 
-    const float* row = p.logits + p.off[u] * V;
-    for (int t = 0; t < (refused ? 0 : T); t++, row += V) {
-        b = s.b[cur];
-        Beams n = s.b[cur ^ 1];
-        // the row: maximum, exp(logit - max), sum
-        float mx = -INFINITY;
-        for (int v = tid; v < V; v += kThreads) mx = fmaxf(mx, clean(row[v]));
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (lane == 0) red_f[warp] = mx;
-        if (tid == 0) { best_key = 0; n_new = 0; n_back = 0; }
-        __syncthreads();
-        for (int i = 0; i < kThreads / 32; i++) mx = fmaxf(mx, red_f[i]);
-        double z = 0.0;
-        for (int v = tid; v < V; v += kThreads) {
-            const float x = clean(row[v]);
-            const double e = x == -INFINITY ? 0.0 : exp((double)x - (double)mx);
-            s.p[v] = e;
-            z += e;
+    const int n_frames = refused ? 0 : T;
+    const float* x = p.logits + p.off[u] * V;
+    const int rbytes = row_bytes(V, W);
+    if (warp >= NC) {
+        int sl = warp - NC;              // slot of the frame, and whether the ring's rounds so far are odd
+        uint32_t odd = 0;
+        for (int t = warp - NC; t < n_frames; t += NP) {
+            const float* row = x + (long long)t * V;
+            float mx = -INFINITY;
+            for (int v = lane; v < V; v += 32) mx = fmaxf(mx, clean(row[v]));
+            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[sl], odd ^ 1u, p.err))) break;
+            make_row(row, V, p.blank, n_tok, mx, row_at(rows + sl * rbytes, V, n_tok));
+            if (lane == 0) mbar_arrive(&full[sl]);
+            sl += NP;
+            if (sl >= p.slots) { sl -= p.slots; odd ^= 1u; }
         }
-        for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-        if (lane == 0) red_d[warp] = z;
-        if (tid < nb && b.par[tid] >= 0)
-            atomicOr(&s.bits[b.par[tid] * s.words + (b.last[tid] >> 5)], 1u << (b.last[tid] & 31));
-        __syncthreads();
-        z = 0.0;
-        for (int i = 0; i < kThreads / 32; i++) z += red_d[i];
-        if (z > 0.0) log_z += log(z);
-        // tokens by probability (equal ones by id)
-        for (int v = tid; v < V; v += kThreads) {
-            if (v == p.blank) continue;
-            const double e = s.p[v];
-            int r = 0;
-            for (int w = 0; w < V; w++) {
-                const double f = s.p[w];
-                r += w != p.blank && (f > e || (f == e && w < v));
+    } else {
+        int pi[kPairs], pj[kPairs];      // this thread's extensions (beam, rank), beam MW: none
+#pragma unroll
+        for (int e = 0; e < kPairs; e++) {
+            const int c = e * NT + tid;
+            pi[e] = c < p.n_pairs ? s.pair[c] >> 8 : MW;
+            pj[e] = c < p.n_pairs ? s.pair[c] & 255 : 0;
+        }
+        int sl = 0, cur = 0;
+        uint32_t odd = 0;
+        bool ready = false;              // the frame's row was seen to be complete
+        for (int t = 0; t < n_frames; t++) {
+            if (!ready && !mbar_wait(&full[sl], odd, p.err)) s.expired = 1;
+            const Row r = row_at(rows + sl * rbytes, V, n_tok);
+            const Beams<MW>& b = s.beams[cur];
+            Beams<MW>& n = s.beams[cur ^ 1];
+            // all that the frame's candidates need, before anything is stored
+            Ranked kr[kPairs];
+            typename Beams<MW>::Prob kq[kPairs];
+            int kl[kPairs];
+            uint32_t kw[kPairs];
+#pragma unroll
+            for (int e = 0; e < kPairs; e++) {
+                const int i = pi[e] < W ? pi[e] : 0;     // beams from nb on hold something, and are left out below
+                kr[e] = r.by_rank[pj[e]];
+                kq[e] = b.prob[i];
+                kl[e] = b.info[i].last;
+                kw[e] = bits[i * words + (kr[e].tok >> 5)] >> (kr[e].tok & 31);
             }
-            if (r < nt) { s.stok[r] = v; s.sp[r] = e; }
-        }
-        __syncthreads();
-        // candidates
-        u64 top = 0;
-        for (int c = tid; c < W + p.n_pairs; c += kThreads) {
-            double val = 0.0;
-            uint32_t ord = 0;
-            if (c < W) {
-                ord = (uint32_t)c;
-                if (c < nb) {
-                    double from = b.pn[c];
-                    const int q = b.par[c];
-                    if (q >= 0) from += b.last[q] == b.last[c] ? b.pb[q] : b.pb[q] + b.pn[q];
-                    val = (b.pb[c] + b.pn[c]) * s.p[p.blank];
-                    if (b.last[c] >= 0) val += from * s.p[b.last[c]];
+            const int me = tid < W ? tid : 0, up = my_par >= 0 ? my_par : 0;
+            const Ranked k0 = r.by_rank[0], k1 = r.by_rank[n_tok > 1 ? 1 : 0];
+            const double p_blank = r.p[p.blank], p_last = r.p[my_last >= 0 ? my_last : 0];
+            const auto above = b.prob[up];
+            const int above_last = b.info[up].last;
+            const uint32_t w0 = bits[me * words + (k0.tok >> 5)] >> (k0.tok & 31);
+            const uint32_t w1 = bits[me * words + (k1.tok >> 5)] >> (k1.tok & 31);
+            // the stays, and each beam's best candidate: `width` different ones, so the
+            // least of them bounds from below what can be kept
+            u64 stay = 0, most = ~(u64)0;
+            if (tid < nb) {
+                const double from = my_par >= 0 ? my_pn + (above_last == my_last ? above.pb : above.total) : my_pn;
+                const double sb = my_total * p_blank, sn = my_last >= 0 ? from * p_last : 0.0;
+                stay = bits_of(sb + sn);
+                most = stay;
+                // no more than two looked at: the likeliest token is as a rule neither a beam's already nor the beam's last
+                const u64 e0 = bits_of((k0.tok == my_last ? my_pb : my_total) * k0.p);
+                const u64 e1 = bits_of((k1.tok == my_last ? my_pb : my_total) * k1.p);
+                if (!(w0 & 1u) && e0 > most) most = e0;
+                if (!(w1 & 1u) && e1 > most) most = e1;
+                s.stay[tid] = {sb, sn};
+                s.slot[tid] = -1;
+            }
+            uint32_t least = __reduce_min_sync(0xffffffffu, (uint32_t)(most >> 32));
+            if (NC > 1 && lane == 0) s.least_hi[warp] = least;
+            // the extensions
+            u64 key[kPairs];
+            uint32_t cand[kPairs];
+#pragma unroll
+            for (int e = 0; e < kPairs; e++) {
+                cand[e] = pack_cand(pi[e], kr[e].tok);
+                const u64 v = bits_of((kr[e].tok == kl[e] ? kq[e].pb : kq[e].total) * kr[e].p);
+                key[e] = pi[e] < nb && !(kw[e] & 1u) ? v : 0;
+            }
+            search_sync<NC>();
+            if (s.expired) break;
+            if (NC > 1) {
+#pragma unroll
+                for (int i = 0; i < NC; i++) least = min(least, s.least_hi[i]);
+            }
+            if (nb < W) least = 0;
+            // those in the running
+            uint32_t in[kPairs + 1];
+            int total_in = 0;
+#pragma unroll
+            for (int e = 0; e <= kPairs; e++) {
+                const u64 k = e < kPairs ? key[e < kPairs ? e : 0] : stay;
+                in[e] = __ballot_sync(0xffffffffu, k >= kLeast && (uint32_t)(k >> 32) >= least);
+                total_in += __popc(in[e]);
+            }
+            if (NC == 1 || total_in) {
+                int at = 0;
+                if (NC > 1) {
+                    if (lane == 0) at = atomicAdd(&s.n_live, total_in);
+                    at = __shfl_sync(0xffffffffu, at, 0);
+                }
+#pragma unroll
+                for (int e = 0; e <= kPairs; e++) {
+                    if (in[e] >> lane & 1u) {
+                        const int pos = at + __popc(in[e] & ((1u << lane) - 1u));
+                        const u64 k = e < kPairs ? key[e < kPairs ? e : 0] : stay;
+                        s.key[pos] = k;
+                        s.key32[pos] = leading(k);
+                        s.cand[pos] = e < kPairs ? cand[e < kPairs ? e : 0] : pack_cand(tid, -1);
+                    }
+                    at += __popc(in[e]);
+                }
+            }
+            search_sync<NC>();
+            const int live = NC == 1 ? total_in : s.n_live;
+            // their places in order: how many have larger leading bits (which decide but for one
+            // frame in some hundreds)
+            auto put = [&](int c, int a) {
+                if (c >= W) return;
+                const uint32_t cd = s.cand[a];
+                s.sel[c] = {s.key[a], cd, 0};
+                if (token_of(cd) < 0) s.slot[beam_of(cd)] = c;
+            };
+            int places = 0;
+            if (NC > 1 && 2 * live <= NT) {      // two threads per candidate, 32 of the others in turn
+                const int a = tid >> 1;
+                int c = 0;
+                if (warp * 16 < live) {
+                    c = count_above(s.key32 + (tid & 1) * 32, live - (tid & 1) * 32, 64, s.key32[a]);
+                    c += __shfl_xor_sync(0xffffffffu, c, 1);
+                }
+                if (a < live && !(tid & 1)) {
+                    places = c;
+                    put(c, a);
                 }
             } else {
-                const int i = s.pair[c - W] >> 8, j = s.pair[c - W] & 255;
-                if (i < nb) {
-                    const int tok = s.stok[j];
-                    ord = (uint32_t)(W + i * V + tok);
-                    if (!(s.bits[i * s.words + (tok >> 5)] >> (tok & 31) & 1u))
-                        val = (tok == b.last[i] ? b.pb[i] : b.pb[i] + b.pn[i]) * s.sp[j];
+                for (int a = tid; a < live; a += NT) {
+                    const int c = count_above(s.key32, live, 32, s.key32[a]);
+                    places += c;
+                    put(c, a);
                 }
             }
-            const u64 k = (u64)__double_as_longlong(val);   // positive numbers order as their bits
-            s.key[c] = k;
-            s.order[c] = ord;
-            top = k > top ? k : top;
-        }
-        atomicMax(&best_key, top);
-        if (tid < W) s.slot[tid] = -1;
-        __syncthreads();
-        // the `width` largest, in order
-        const double best = __longlong_as_double((long long)best_key);
-        const u64 least = (u64)__double_as_longlong(fmax(best * 0x1p-1000, DBL_MIN));
-        for (int c = tid; c < W + p.n_pairs; c += kThreads) {
-            const u64 k = s.key[c];
-            if (k < least) continue;
-            const uint32_t o = s.order[c];
-            int r = 0;
-            for (int d = 0; d < W + p.n_pairs; d++) r += s.key[d] > k || (s.key[d] == k && s.order[d] < o);
-            if (r < W) {
-                s.sel[r] = c;
-                if (c < W) s.slot[c] = r;
-                atomicMax(&n_new, r + 1);
-            }
-        }
-        if (tid < nb && b.par[tid] >= 0) s.bits[b.par[tid] * s.words + (b.last[tid] >> 5)] = 0;
-        __syncthreads();
-        // the new beams
-        const int e2 = best > 0.0 ? ilogb(best) : 0;
-        const double scale = scalbn(1.0, -e2);
-        const int nn = n_new;
-        int fresh = -1;          // the old beam whose new child this thread's beam is
-        if (tid < nn) {
-            const int c = s.sel[tid];
-            if (c < W) {
-                double from = b.pn[c];
-                const int q = b.par[c];
-                if (q >= 0) from += b.last[q] == b.last[c] ? b.pb[q] : b.pb[q] + b.pn[q];
-                n.pb[tid] = (b.pb[c] + b.pn[c]) * s.p[p.blank] * scale;
-                n.pn[tid] = b.last[c] >= 0 ? from * s.p[b.last[c]] * scale : 0.0;
-                n.node[tid] = b.node[c];
-                n.last[tid] = b.last[c];
-                n.len[tid] = b.len[c];
-                n.pnode[tid] = b.pnode[c];
-            } else {
-                const int i = s.pair[c - W] >> 8, tok = s.stok[s.pair[c - W] & 255];
-                int id = -1;
-                if (b.mask[i] >> (tok & 63) & 1)
-                    for (id = b.head[i]; id >= 0 && nodes[id].tok != tok; id = nodes[id].next) {}
-                if (id >= 0) {   // reached again after it was dropped
-                    n.head[tid] = nodes[id].head;
-                    n.mask[tid] = masks[id];
-                    s.back[atomicAdd(&n_back, 1)] = tid;
-                } else {
-                    id = 1 + (frames + t) * W + tid;
-                    n.head[tid] = -1;
-                    n.mask[tid] = 0;
-                    fresh = i;
+            // equal ones take one place: the places add up to less than 0 + 1 + .. + live - 1
+            auto all_differ = [&]() {
+                places = __reduce_add_sync(0xffffffffu, places);
+                if (NC > 1 && lane == 0) atomicAdd(&s.place_sum, places);
+                search_sync<NC>();
+                return (NC > 1 ? s.place_sum : places) == live * (live - 1) / 2;
+            };
+            if (!all_differ()) {
+                // by the whole values
+                search_sync<NC>();
+                if (tid < nb) s.slot[tid] = -1;
+                if (tid == 0) s.place_sum = 0;
+                search_sync<NC>();
+                places = 0;
+                for (int a = tid; a < live; a += NT) {
+                    const u64 k = s.key[a];
+                    int c = 0;
+#pragma unroll 8
+                    for (int d = 0; d < live; d++) c += s.key[d] > k;
+                    places += c;
+                    put(c, a);
                 }
-                n.pb[tid] = 0.0;
-                n.pn[tid] = __longlong_as_double((long long)s.key[c]) * scale;
-                n.node[tid] = id;
-                n.last[tid] = tok;
-                n.len[tid] = b.len[i] + 1;
-                n.pnode[tid] = b.node[i];
+                if (!all_differ()) {
+                    // and the rule for equal ones: stays first, then by beam and token
+                    if (tid < nb) s.slot[tid] = -1;
+                    search_sync<NC>();
+                    auto order = [&](uint32_t c) {
+                        return token_of(c) < 0 ? beam_of(c) : W + beam_of(c) * V + token_of(c);
+                    };
+                    for (int a = tid; a < live; a += NT) {
+                        const u64 k = s.key[a];
+                        const int o = order(s.cand[a]);
+                        int c = 0;
+                        for (int d = 0; d < live; d++) c += s.key[d] > k || (s.key[d] == k && order(s.cand[d]) < o);
+                        put(c, a);
+                    }
+                    search_sync<NC>();
+                }
             }
-        }
-        __syncthreads();
-        if (fresh >= 0) {
-            const int tok = n.last[tid], id = n.node[tid];
-            nodes[id] = Node{b.node[fresh], tok, -1, atomicExch(&b.head[fresh], id)};
-            atomicOr(&b.mask[fresh], (u64)1 << (tok & 63));
-        }
-        __syncthreads();
-        if (tid < nb) {
-            const int r = s.slot[tid];
-            if (r >= 0) {
-                n.head[r] = b.head[tid];
-                n.mask[r] = b.mask[tid];
-            } else {
-                nodes[b.node[tid]].head = b.head[tid];
-                masks[b.node[tid]] = b.mask[tid];
+            // the new beams, but those below 2^-1000 of the best
+            int nn = min(live, W);
+            const u64 best = nn ? s.sel[0].key : 0;
+            const int e2 = nn ? (int)(best >> 52) - 1023 : 0;
+            const double scale = value_of((u64)(1023 - e2) << 52);
+            const u64 floor = best > ((u64)1000 << 52) ? best - ((u64)1000 << 52) : 0;
+            while (nn && s.sel[nn - 1].key < floor) nn--;
+            const int my_slot = tid < nb ? s.slot[tid] : 0;
+            const bool drops = tid < nb && (uint32_t)my_slot >= (uint32_t)nn;
+            if (tid < nb && my_par >= 0) bits[my_par * words + (my_last >> 5)] = 0;
+            int fresh = -1;          // the old beam whose new child this thread's beam is
+            int my_node = 0, my_pnode = 0;
+            if (tid < nn) {
+                const auto c = s.sel[tid];
+                const int i = beam_of(c.cand), tk = token_of(c.cand);
+                const bool stays = tk < 0;
+                const auto info = b.info[i];
+                const auto link = b.link[i];
+                const auto held = s.stay[i];
+                const int from = stays ? link.par : i;           // old place of the parent
+                int par = s.slot[from >= 0 ? from : 0];
+                if (from < 0 || par >= nn) par = -1;
+                uint32_t mask0 = link.mask[0], mask1 = link.mask[1];
+                int head = link.head;
+                my_node = info.node;
+                if (!stays) {
+                    int id = -1;
+                    if ((tk & 32 ? mask1 : mask0) >> (tk & 31) & 1u)
+                        for (id = head; id >= 0 && nodes[id].tok != tk; id = nodes[id].next) {}
+                    if (id >= 0) {   // reached again after it was dropped
+                        head = nodes[id].head;
+                        mask0 = (uint32_t)masks[id];
+                        mask1 = (uint32_t)(masks[id] >> 32);
+                        s.back[atomicAdd(&s.n_back, 1)] = tid;
+                    } else {
+                        id = 1 + (frames + t) * W + tid;
+                        head = -1;
+                        mask0 = mask1 = 0;
+                        fresh = i;
+                    }
+                    my_node = id;
+                }
+                my_pnode = stays ? info.pnode : info.node;
+                my_last = stays ? info.last : tk;
+                my_pb = stays ? held.b * scale : 0.0;
+                my_pn = (stays ? held.n : value_of(c.key)) * scale;
+                my_total = my_pb + my_pn;
+                my_par = par;
+                n.prob[tid] = {my_pb, my_total};
+                n.pn[tid] = my_pn;
+                n.info[tid] = {my_node, my_last, info.len + !stays, my_pnode};
+                n.link[tid] = {{mask0, mask1}, head, par};
             }
+            for (int a = tid; a < live; a += NT) s.key32[a] = 0;
+            if (tid == 0) log_z += *r.log_z;
+            search_sync<NC>();
+            if (tid == 0) {
+                mbar_arrive(&empty[sl]);
+                s.n_live = 0;
+                s.place_sum = 0;
+            }
+            const int nback = s.n_back;
+            // children join their parents' lists (a parent that drops: its old place's), and mark them
+            if (fresh >= 0) {
+                auto& parent = my_par >= 0 ? n.link[my_par] : s.beams[cur].link[fresh];
+                nodes[my_node] = Node{my_pnode, my_last, -1, atomicExch(&parent.head, my_node)};
+                atomicOr(&parent.mask[my_last >> 5 & 1], 1u << (my_last & 31));
+            }
+            if (tid < nn) {
+                if (nback && my_par < 0)
+                    for (int i = 0; i < nback; i++)
+                        if (n.info[s.back[i]].node == my_pnode) n.link[tid].par = my_par = s.back[i];
+                if (my_par >= 0) atomicOr(&bits[my_par * words + (my_last >> 5)], 1u << (my_last & 31));
+            }
+            search_sync<NC>();
+            if (drops) {
+                const int id = b.info[tid].node;
+                nodes[id].head = b.link[tid].head;
+                masks[id] = (u64)b.link[tid].mask[1] << 32 | b.link[tid].mask[0];
+            }
+            if (tid == 0) s.n_back = 0;
+            exp2 += e2;
+            nb = nn;
+            cur ^= 1;
+            if (++sl == p.slots) { sl = 0; odd ^= 1u; }
+            ready = t + 1 < n_frames && mbar_try_wait(&full[sl], odd);
         }
-        if (tid < nn) {
-            const int c = s.sel[tid];
-            const int q = c < W ? b.par[c] : s.pair[c - W] >> 8;
-            int par = q >= 0 ? s.slot[q] : -1;
-            if (par < 0 && c < W)
-                for (int i = 0; i < n_back; i++)
-                    if (n.node[s.back[i]] == n.pnode[tid]) par = s.back[i];
-            n.par[tid] = par;
-        }
-        exp2 += e2;
-        nb = nn;
-        cur ^= 1;
-        __syncthreads();
-    }
-    b = s.b[cur];
-
-    // state for the next call
-    if (!refused) {
+        search_sync<NC>();
+        const bool failed = s.expired != 0;  // a wait ran out (reported by mbar_wait)
         if (tid == 0) {
-            hdr->frames = frames + T;
-            hdr->nb = nb;
-            hdr->tag = tag;
-            hdr->exp2 = exp2;
-            hdr->log_z = log_z;
+            s.nb = refused || failed ? 0 : nb;
+            s.cur = cur;
+            s.exp2 = exp2;
+            s.log_z = log_z;
+            if (failed) hdr->tag = 0;
         }
-        if (tid < nb) {
-            saved.pb[tid] = b.pb[tid];
-            saved.pn[tid] = b.pn[tid];
-            saved.mask[tid] = b.mask[tid];
-            saved.node[tid] = b.node[tid];
-            saved.last[tid] = b.last[tid];
-            saved.len[tid] = b.len[tid];
-            saved.pnode[tid] = b.pnode[tid];
-            saved.par[tid] = b.par[tid];
-            saved.head[tid] = b.head[tid];
+        // state for the next call
+        if (!refused && !failed) {
+            if (tid == 0) {
+                hdr->frames = frames + T;
+                hdr->nb = nb;
+                hdr->tag = tag;
+                hdr->exp2 = exp2;
+                hdr->log_z = log_z;
+            }
+            if (tid < nb) {
+                const auto info = s.beams[cur].info[tid];
+                const auto link = s.beams[cur].link[tid];
+                saved[tid] = SavedBeam{my_pb, my_pn, (u64)link.mask[1] << 32 | link.mask[0], info.node, info.last, info.len, info.pnode, link.par, link.head};
+            }
         }
     }
+    if (p.n_best == 0) return;
+    __syncthreads();
     // hypotheses, best first
-    const int have = refused ? 0 : nb < p.n_best ? nb : p.n_best;
-    for (int h = warp; h < p.n_best; h += kThreads / 32) {
+    const Beams<MW>& b = s.beams[s.cur];
+    const int have = s.nb < p.n_best ? s.nb : p.n_best;
+    for (int h = warp; h < p.n_best; h += NC + NP) {
         const long long at = (long long)u * p.n_best + h;
-        const int len = h < have ? b.len[h] : -1;
+        const int len = h < have ? b.info[h].len : -1;
         int* out = p.ids + at * p.cap;
         for (long long i = (len > 0 ? len : 0) + lane; i < p.cap; i += 32) out[i] = -1;
         if (lane) continue;
         p.n_ids[at] = len;
-        p.scores[at] = h < have ? log(b.pb[h] + b.pn[h]) + (double)exp2 * 0.69314718055994530942 - log_z
-                                : -INFINITY;
+        p.scores[at] = h < have ? log(b.prob[h].total) + (double)s.exp2 * 0.69314718055994530942 - s.log_z : -INFINITY;
         if (len > 0)
-            for (int i = len - 1, id = b.node[h]; i >= 0; i--, id = nodes[id].parent)
-                if (i < p.cap) out[i] = nodes[id].tok;
+            for (int i = len - 1, id = b.info[h].node; i >= 0; i--) {
+                const Node nd = nodes[id];
+                if (i < p.cap) out[i] = nd.tok;
+                id = nd.parent;
+            }
     }
+}
+
+template <int NC, int NP, int MW>
+static int launch(Params p, int n_utt, cudaStream_t st) {
+    const long long fixed = (long long)sizeof(Shared<MW>) + (p.width * ((p.V + 31) / 32) * 4 + 15) / 16 * 16;
+    const long long row = row_bytes(p.V, p.width);
+    p.slots = fixed + 2 * NP * row <= 200 * 1024 ? 2 * NP : NP;
+    const long long smem = fixed + p.slots * row;
+    static bool attr[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    auto kern = ctc_beam_kernel<NC, NP, MW>;
+    if (!attr[dev & 63]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess)
+            return W2V_ERR_LAUNCH;
+        attr[dev & 63] = true;
+    }
+    kern<<<n_utt, (NC + NP) * 32, smem, st>>>(p);
+    return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
 
 }  // namespace cb
@@ -470,10 +680,7 @@ extern "C" int w2v_ctc_beam(const float* logits, const long long* off, const int
     p.err = err;
     p.n_pairs = 0;
     for (int i = 0; i < width; i++) p.n_pairs += pairs_of(i, V, width);
-    const int smem = (int)smem_layout(nullptr, nullptr, V, width, p.n_pairs);
-    if (smem > 40 * 1024 &&          // beside the static part
-        cudaFuncSetAttribute(ctc_beam_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return W2V_ERR_LAUNCH;
-    ctc_beam_kernel<<<n_utt, kThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-    return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    // up to 32 beams one warp searches, without barriers
+    return width <= 32 ? launch<1, 4, 32>(p, n_utt, st) : launch<8, 8, 128>(p, n_utt, st);
 }
