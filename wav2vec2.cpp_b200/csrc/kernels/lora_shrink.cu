@@ -3,199 +3,428 @@
 // (segments.cuh).
 //
 // 2 M K rank operations on M K fp16 values: with the ranks in use (8 .. 128)
-// the read of x bounds it.  A block of 128 threads takes 64 rows (of one row
-// tile) and K in steps of 64 through a ring of shared-memory stages filled by
-// cp.async; each warp multiplies 16 rows by all `rank` rows of A_a with
-// m16n8k16 instructions, fp32 accumulators in registers.  Several blocks per
-// SM keep some 100 KB of x in flight.  A row tile used by several adapters is
-// done once per adapter, by blockIdx.y in turn, where any of the 64 rows use it.
+// the read of x bounds it, and the time from a block's start to its end where
+// there are few rows.  A block takes 128 rows, or 64 where those are few or the
+// row tile is no multiple of 128 (the MMA's other 64 rows are then whatever lies
+// behind them).  A ring of stages holds 64 columns of x and of A_a; a warp of its
+// own fills it by TMA, x at once and A_a when the other four have looked the
+// block's adapters up.  tcgen05.mma multiplies a stage by each of two adapters, if
+// the rows use two, into accumulators side by side in TMEM, so that a block that
+// sees the end of an utterance takes hardly longer than the others.  (With
+// m16n8k16 MMAs in registers their rate was the bound: 60 x 10 s, K 1024, rank 64
+// took 31 us.)  More adapters (single frames) are taken in turn, by other
+// blocks where there are few rows.
 #include "segments.cuh"
 #include "w2v_kernels.h"
 
 namespace w2v {
 namespace sg {
 
-constexpr int kRows = 64, kStep = 64, kThreads = 128, kMaxTile = 256;
+constexpr int kStep = 64, kMaxTile = 256;
+constexpr int kPlanners = 128, kThreads = kPlanners + 32;
+constexpr int kMaxRing = 8;
 
-__host__ __device__ constexpr int stage_bytes(int rank) { return (kRows + rank) * kStep * 2; }
-
-// 16-byte group g of row r of a [rows][64] fp16 tile, 128-byte rows, groups
-// XOR-swizzled by row so that both the copies and ldmatrix are conflict free.
-W2V_DEV uint32_t tile_at(uint32_t base, int r, int g) { return base + (uint32_t)(r * 128 + ((g ^ (r & 7)) << 4)); }
-
-W2V_DEV void cp_async16_zfill(uint32_t saddr, const void* g, bool real) {
-    const int n = real ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(g), "r"(n) : "memory");
+struct ShrinkShape {
+    int stages, stage_bytes, smem;
+    int split, cols;       // accumulators of an adapter; columns of TMEM
+};
+// Two blocks per SM where a ring of three stages or more allows it.  An MMA of
+// few columns waits longer for the one before it on the same accumulator than it
+// takes (some 200 cycles at 16), so the MMAs of a stage go to up to four
+// accumulators in turn, which the epilogue adds: 64 x 10 s, K 768, rank 16 X us.
+static ShrinkShape shrink_shape(int rows, int rank) {
+    ShrinkShape s;
+    s.stage_bytes = (rows + 2 * rank) * kStep * 2;
+    const int behind = 64 * kStep * 2 + 1024;  // what the last stage's MMAs may read past it
+    const int two = (108 * 1024 - behind) / s.stage_bytes, one = (216 * 1024 - behind) / s.stage_bytes;
+    s.stages = two >= 3 ? two : one;
+    if (s.stages > kMaxRing) s.stages = kMaxRing;
+    s.smem = 1024 + s.stages * s.stage_bytes + behind + 256;
+    const int n16 = (rank + 15) / 16 * 16;
+    s.split = n16 <= 32 ? 4 : n16 <= 64 ? 2 : 1;
+    s.cols = 32;
+    while (s.cols < 2 * s.split * n16) s.cols *= 2;
+    return s;
 }
 
-template <int NT>   // rank / 8
-__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(LoraArgs a, LoraPlan p, int stages) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int row_adapter[kMaxTile];
+// Barriers of the four warps that plan.
+W2V_DEV void plan_sync() { asm volatile("barrier.sync 1, 128;" ::: "memory"); }
+W2V_DEV int plan_count(bool x) {
+    int n;
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.s32 p, %1, 0;\n barrier.red.popc.u32 %0, 1, 128, p;\n}"
+        : "=r"(n)
+        : "r"((int)x)
+        : "memory");
+    return n;
+}
+
+template <int kRows>
+__global__ void __launch_bounds__(kThreads)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, LoraArgs a, LoraPlan p,
+                   ShrinkShape shape) {
+    constexpr int kXBytes = kRows * kStep * 2;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint16_t seg_start[kMaxTile], seg_end[kMaxTile];   // the tile's utterances that have rows in it
+    __shared__ __align__(16) int seg_adapter[kMaxTile];
+    __shared__ int16_t seg_slot[kMaxTile];
     __shared__ int slots[kMaxTile];           // the tile's adapters, by their first row
-    __shared__ int n_slots;
-    constexpr int rank = NT * 8;
+    __shared__ int16_t here[kMaxTile];        // those of them that this block's rows use, then the others
+    __shared__ uint8_t present[kMaxTile];
+    __shared__ uint32_t present_mask;
+    __shared__ int counts[kPlanners / 32];
+    __shared__ int row_slot[128];             // of this block's rows
+    __shared__ int n_here_shared;
+    __shared__ long long first_block_shared;
+    __shared__ uint64_t full[kMaxRing], empty[kMaxRing], done;
+    __shared__ uint32_t tmem_slot;
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t* ring = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    const int S = shape.stages, split = shape.split;
+    const int rank = p.rank, n16 = (rank + 15) / 16 * 16, a_bytes = rank * kStep * 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    grid_launch_dependents();
     const long long row0 = (long long)blockIdx.x * kRows;
     const long long tile = row0 / p.tile;
     const long long tile0 = tile * p.tile;
     const int n_rows = (int)min((long long)p.tile, a.M - tile0);
-
-    // adapters of the tile's rows
-    auto adapter_of = [&](int u) {
-        const int v = u < 0 ? -1 : a.adapter[u];
-        return v >= 0 && v < a.n_adapters ? v : -1;
-    };
-    for (int i = tid; i < n_rows; i += kThreads)
-        row_adapter[i] = adapter_of(utterance_of(a.off, a.T, a.n_utt, tile0 + i));
-    if (tid == 0) n_slots = 0;
-    __syncthreads();
-    for (int i0 = 0; i0 < n_rows; i0 += kThreads) {
-        const int i = i0 + tid;
-        bool first = false;
-        if (i < n_rows) {
-            const int v = row_adapter[i];
-            first = v >= 0 && (i == 0 || row_adapter[i - 1] != v);
-            for (int j = 0; first && j < i; j++) first = row_adapter[j] != v;
-        }
-        __shared__ int base[kThreads / 32];
-        const uint32_t m = __ballot_sync(0xffffffffu, first);
-        if (lane == 0) base[warp] = __popc(m);
-        __syncthreads();
-        int at = n_slots;
-        for (int w = 0; w < warp; w++) at += base[w];
-        if (first) slots[at + __popc(m & ((1u << lane) - 1u))] = row_adapter[i];
-        __syncthreads();
-        if (tid == kThreads - 1) n_slots = at + __popc(m);
-        __syncthreads();
-    }
-    const int count = n_slots;
-    // first block of the tile
-    int lo = 0, hi = a.n_utt;                 // utterances that start before the tile
-    while (lo < hi) {
-        const int m = (lo + hi) / 2;
-        if (a.off[m] < tile0) lo = m + 1; else hi = m;
-    }
-    const long long first_block = tile + (lo < tile0 ? lo : tile0);
-    if (row0 == tile0 && blockIdx.y == 0) {
-        if (tid == 0) p.tiles[tile] = LoraTile{(int)first_block, count};
-        for (int i = tid; i < count; i += kThreads) p.adapter[first_block + i] = slots[i];
-    }
-
-    const int k_steps = a.K / kStep;
-    const uint32_t sbase = smem_u32(smem);
     const int local0 = (int)(row0 - tile0);
-    for (int s = blockIdx.y; s < count; s += gridDim.y) {
-        const int ad = slots[s];
-        bool mine = false;                    // any of the 64 rows
-        if (tid < kRows && local0 + tid < n_rows) mine = row_adapter[local0 + tid] == ad;
-        const bool some = __syncthreads_or(mine);
-        float acc[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[n][i] = 0.f;
-        if (some) {
-            const __half* wa = a.a + (long long)ad * rank * a.K;
-            auto fetch = [&](int ks) {
-                const uint32_t st = sbase + (uint32_t)((ks % stages) * stage_bytes(rank));
-                const int k0 = ks * kStep;
-#pragma unroll
-                for (int i = 0; i < kRows * 8 / kThreads; i++) {
-                    const int c = tid + i * kThreads, r = c >> 3, g = c & 7;
-                    const bool real = row0 + r < a.M;
-                    cp_async16_zfill(tile_at(st, r, g), a.x + (real ? row0 + r : 0) * a.lda + k0 + g * 8, real);
-                }
-                for (int c = tid; c < rank * 8; c += kThreads) {
-                    const int r = c >> 3, g = c & 7;
-                    cp_async16(tile_at(st + kRows * kStep * 2, r, g), wa + (long long)r * a.K + k0 + g * 8);
-                }
-            };
-            for (int ks = 0; ks < stages - 1; ks++) {
-                if (ks < k_steps) fetch(ks);
-                cp_async_commit();
+    const int k_steps = a.K / kStep;
+    const long long part = p.blocks * p.tile * rank;
+    // the block that is sure to use its rows fetches the first of them before it knows the adapters
+    const int early = blockIdx.y == 0 ? min(S, k_steps) : 0;
+
+    // a stage's x (and the adapters' share) arrives on full[st]: two arrivals
+    const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), lead = elect_one();
+    auto load_x = [&](int st, int ks) {
+        expect_tx_if(lead, full0 + (uint32_t)(st * 8), kXBytes);
+        tma_load_2d_if<false>(lead, ring0 + (uint32_t)(st * shape.stage_bytes), &tmX, full0 + (uint32_t)(st * 8), ks * kStep,
+                              (int)row0);
+    };
+    if (warp == kPlanners / 32) {
+        if (lane == 0) {
+            for (int s = 0; s < S; s++) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
+            mbar_init(&done, 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+        for (int ks = 0; ks < early; ks++) load_x(ks, ks);
+    }
+    if (warp == 0) {
+        // TMEM first: a projection's block that came to this SM before would hold all of it
+        // while it waits for this grid
+        tmem_alloc(&tmem_slot, shape.cols);
+        tmem_relinquish();
+        grid_launch_dependents();
+    }
+
+    if (warp < kPlanners / 32) {
+        if (tid == 0) present_mask = 0;
+        auto end_of = [&](int u) { return a.off[u] + max(a.T[u], 0); };
+
+        // utterances that end before the tile: ends ascend, kPlanners of them looked at at a time
+        int lo = 0, hi = a.n_utt;
+        while (hi - lo > kPlanners) {
+            const int step = (hi - lo + kPlanners - 1) / kPlanners;
+            const int u = lo + tid * step;
+            const int n = plan_count(u < hi && end_of(u) <= tile0);
+            if (n == 0) { hi = lo; break; }
+            hi = min(hi, lo + n * step);          // the n-th looked at does not end before
+            lo += (n - 1) * step + 1;
+        }
+        // the rest of them, and the utterances in the tile
+        int n_seg = 0, ended = lo;
+        for (int u0 = lo; u0 < a.n_utt; u0 += kPlanners) {
+            const int u = u0 + tid;
+            long long start = 0, end = 0;
+            bool in = false, past = false, before = false;
+            int ad = -1;
+            if (u < a.n_utt) {
+                start = a.off[u];
+                past = start >= tile0 + n_rows;
+                const int len = a.T[u], v = a.adapter[u];
+                before = start + max(len, 0) <= tile0;
+                in = !past && !before && len > 0;
+                end = min(start + len - tile0, (long long)n_rows);
+                ad = v >= 0 && v < a.n_adapters ? v : -1;
             }
+            const uint32_t m = __ballot_sync(0xffffffffu, in);
+            if (lane == 0) counts[warp] = __popc(m);
+            plan_sync();
+            int at = n_seg;
+            for (int w = 0; w < kPlanners / 32; w++) {
+                if (w < warp) at += counts[w];
+                n_seg += counts[w];
+            }
+            at += __popc(m & ((1u << lane) - 1u));
+            if (in && at < kMaxTile) {
+                seg_start[at] = (uint16_t)max(start - tile0, 0LL);
+                seg_end[at] = (uint16_t)end;
+                seg_adapter[at] = ad;
+            }
+            ended += plan_count(before);
+            if (u0 + kPlanners < a.n_utt && plan_count(past)) break;
+        }
+        n_seg = min(n_seg, kMaxTile);
+        const long long first_block = tile + (ended < tile0 ? ended : tile0);
+        int count = 0, n_here = 0;
+        if (n_seg <= 32) {
+            // by every warp for itself: each adapter once, and the row's
+            const int v = lane < n_seg ? seg_adapter[lane] : -1;
+            const int from = lane < n_seg ? seg_start[lane] : 0, to = lane < n_seg ? seg_end[lane] : 0;
+            const uint32_t same = __match_any_sync(0xffffffffu, v);
+            const bool first = v >= 0 && __ffs(same) - 1 == lane;
+            const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+            const int at = __popc(firsts & ((1u << lane) - 1u));
+            int slot = __shfl_sync(0xffffffffu, at, __ffs(same) - 1);
+            // (utterances that overlap or are out of order must not lead out of the plan)
+            count = (int)min((long long)__popc(firsts), max(p.blocks - first_block, 0LL));
+            if (v < 0 || slot >= count) slot = -1;
+            if (first && warp == 0) slots[at] = v;
+            int mine = -1;
+            for (int s = 0; s < n_seg; s++) {
+                const int f = __shfl_sync(0xffffffffu, from, s), e = __shfl_sync(0xffffffffu, to, s);
+                const int q = __shfl_sync(0xffffffffu, slot, s);
+                if (local0 + tid >= f && local0 + tid < e) mine = q;
+            }
+            if (tid >= kRows) mine = -1;
+            row_slot[tid] = mine;
+            const uint32_t m = __reduce_or_sync(0xffffffffu, mine >= 0 ? 1u << mine : 0u);
+            if (lane == 0 && m) atomicOr(&present_mask, m);
+            plan_sync();
+            const uint32_t pm = present_mask;
+            n_here = __popc(pm);
+            if (warp == 0 && lane < count) {
+                const int before = __popc(pm & ((1u << lane) - 1u));
+                here[pm >> lane & 1u ? before : count - 1 - (lane - before)] = (int16_t)lane;
+            }
+        } else {
+            // each adapter once
+            for (int i0 = 0; i0 < n_seg; i0 += kPlanners) {
+                const int i = i0 + tid;
+                int j = 0;                            // the first segment of this adapter
+                if (i < n_seg) {
+                    const int v = seg_adapter[i];
+                    while (j + 4 <= i) {
+                        const int4 q = *reinterpret_cast<const int4*>(seg_adapter + j);
+                        if (q.x == v || q.y == v || q.z == v || q.w == v) break;
+                        j += 4;
+                    }
+                    while (j < i && seg_adapter[j] != v) j++;
+                }
+                const bool first = i < n_seg && j == i && seg_adapter[i] >= 0;
+                const uint32_t m = __ballot_sync(0xffffffffu, first);
+                plan_sync();                      // counts are read
+                if (lane == 0) counts[warp] = __popc(m);
+                plan_sync();
+                int at = count;
+                for (int w = 0; w < kPlanners / 32; w++) {
+                    if (w < warp) at += counts[w];
+                    count += counts[w];
+                }
+                at += __popc(m & ((1u << lane) - 1u));
+                if (first) slots[at] = seg_adapter[i];
+                if (i < n_seg && j == i) seg_slot[i] = (int16_t)(first ? at : -1);
+                plan_sync();
+                if (i < n_seg && j != i) seg_slot[i] = seg_slot[j];
+            }
+            plan_sync();
+            count = (int)min((long long)count, max(p.blocks - first_block, 0LL));
+            {
+                int l = 0, h = n_seg;                 // the last segment that starts at or before the row, if it has it
+                while (l < h) {
+                    const int m = (l + h) / 2;
+                    if (seg_start[m] <= local0 + tid) l = m + 1; else h = m;
+                }
+                const int sl = tid < kRows && l > 0 && local0 + tid < seg_end[l - 1] ? seg_slot[l - 1] : -1;
+                row_slot[tid] = sl < count ? sl : -1;
+            }
+            for (int i = tid; i < count; i += kPlanners) present[i] = 0;
+            plan_sync();
+            if (row_slot[tid] >= 0) present[row_slot[tid]] = 1;
+            for (int i0 = 0; i0 < count; i0 += kPlanners) {
+                plan_sync();
+                const int i = i0 + tid;
+                const bool is = i < count && present[i];
+                const uint32_t m = __ballot_sync(0xffffffffu, is);
+                if (lane == 0) counts[warp] = __popc(m);
+                plan_sync();
+                int at = n_here;
+                for (int w = 0; w < kPlanners / 32; w++) {
+                    if (w < warp) at += counts[w];
+                    n_here += counts[w];
+                }
+                at += __popc(m & ((1u << lane) - 1u));
+                if (is) here[at] = (int16_t)i;
+                else if (i < count) here[count - 1 - (i - at)] = (int16_t)i;     // i - at: those absent before it
+            }
+        }
+        plan_sync();
+        if (row0 == tile0 && blockIdx.y == 0) {
+            if (tid == 0) { p.tiles[tile].first = (int)first_block; p.tiles[tile].count = count; }
+            for (int i = tid; i < count; i += kPlanners) {
+                if (i < kInline) p.tiles[tile].adapter[i] = slots[i];
+                p.adapter[first_block + i] = slots[i];
+            }
+        }
+        if (blockIdx.y == 0)                      // the others' blocks are zero in these rows
+            for (int k = n_here; k < count; k++) {
+                __half* out = p.t + ((first_block + here[k]) * p.tile + local0) * rank;
+                const int n = min(kRows, n_rows - local0) * rank / 8;
+                for (int c = tid; c < n; c += kPlanners) {
+                    reinterpret_cast<uint4*>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
+                    if (p.parts == 2) reinterpret_cast<uint4*>(out + part)[c] = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+        if (tid == 0) { n_here_shared = n_here; first_block_shared = first_block; }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int n_here = n_here_shared;
+    const long long first_block = first_block_shared;
+
+    // two adapters a pass; the ring's counters run on
+    const uint32_t tmem = tmem_slot;
+    if (warp == kPlanners / 32) {
+        int st = 0, used = 0;                 // used: stages filled so far
+        uint32_t odd = 0, issued = 0;
+        bool ok = true;
+        for (int base = 2 * blockIdx.y; base < n_here && ok; base += 2 * gridDim.y) {
+            const int n = min(2, n_here - base);
+            const int ad0 = slots[here[base]], ad1 = n > 1 ? slots[here[base + 1]] : 0;
+            const uint32_t second = n > 1 ? lead : 0u;
             for (int ks = 0; ks < k_steps; ks++) {
-                // stage ks has landed when at most stages - 2 younger groups are under way
-                if (stages == 4) cp_async_wait<2>(); else cp_async_wait<1>();
-                __syncthreads();
-                if (ks + stages - 1 < k_steps) fetch(ks + stages - 1);
-                cp_async_commit();
-                const uint32_t sx = sbase + (uint32_t)((ks % stages) * stage_bytes(rank)), sa = sx + kRows * kStep * 2;
+                if (used >= S && !mbar_wait_warp(&empty[st], odd ^ 1u, a.err)) { ok = false; break; }
+                if (used >= early) load_x(st, ks);
+                const uint32_t sa = ring0 + (uint32_t)(st * shape.stage_bytes + kXBytes), bar = full0 + (uint32_t)(st * 8);
+                expect_tx_if(lead, bar, (uint32_t)(n * a_bytes));
+                tma_load_3d_if<false>(lead, sa, &tmA, bar, ks * kStep, 0, ad0);
+                tma_load_3d_if<false>(second, sa + (uint32_t)a_bytes, &tmA, bar, ks * kStep, 0, ad1);
+                issued |= 1u << st;
+                used++;
+                if (++st == S) { st = 0; odd ^= 1u; }
+            }
+        }
+        // no bulk copy may still be writing shared memory when the block exits: rows that
+        // no adapter came for, and what the MMAs have not waited for
+        for (int s = used; s < early; s++) {
+            if (lane == 0) mbar_arrive(&full[s]);
+            mbar_wait(&full[s], 0, a.err);
+        }
+        for (int s = 0; s < S; s++)
+            if (issued >> s & 1u) mbar_wait(&full[s], s < st ? odd : odd ^ 1u, a.err);
+        __syncwarp();
+    } else {
+        int st = 0, pass = 0;
+        uint32_t odd = 0;
+        bool ok = true;
+        for (int base = 2 * blockIdx.y; base < n_here; base += 2 * gridDim.y, pass++) {
+            const int n = min(2, n_here - base);
+            if (warp == 0) {
+                const uint32_t idesc = umma_idesc_f16(128, n16);
+                const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
+                for (int ks = 0; ks < k_steps && ok; ks++) {
+                    if (!mbar_wait_warp(&full[st], odd, a.err)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t dx = desc_plus(desc0, (uint32_t)(st * shape.stage_bytes));
+                    for (int e = 0; e < n; e++) {
+                        const uint64_t db = desc_plus(dx, (uint32_t)(kXBytes + e * a_bytes));
+                        const uint32_t d = tmem + (uint32_t)(e * split * n16);
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++) {
-                    uint32_t x0, x1, x2, x3;
-                    ldsm_x4(tile_at(sx, warp * 16 + (lane & 15), kk * 2 + (lane >> 4)), x0, x1, x2, x3);
+                        for (int kk = 0; kk < kStep / 16; kk++)
+                            umma_f16_if<false>(lead, d + (uint32_t)((kk & (split - 1)) * n16), desc_plus(dx, kk * 32),
+                                               desc_plus(db, kk * 32), idesc, ks != 0 || kk >= split);
+                    }
+                    umma_commit_if<false>(lead, smem_u32(&empty[st]));
+                    if (++st == S) { st = 0; odd ^= 1u; }
+                }
+                umma_commit_if<false>(lead, smem_u32(&done));     // (also after an expired wait)
+            }
+            mbar_wait(&done, (uint32_t)pass & 1u, a.err);
+            tc_fence_after();
+            // masked, as fp16 (and what the rounding left, for fp32 outputs): a row per lane
+            const int r = warp * 32 + lane;
+            if (warp * 32 < kRows) {
+                const bool real = local0 + r < n_rows;
+                const int mine = row_slot[r];
+                for (int e = 0; e < n; e++) {
+                    const int s = here[base + e];
+                    const float sc = a.scale ? a.scale[slots[s]] : 1.f;
+                    __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * rank;
+                    for (int c = 0; c < rank; c += 16) {
+                        float v[16];
+                        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * split * n16 + c);
+                        tmem_ld16(at, v);
+                        for (int q = 1; q < split; q++) {
+                            float w[16];
+                            tmem_ld16(at + (uint32_t)(q * n16), w);
 #pragma unroll
-                    for (int n = 0; n < NT; n += 2) {
-                        uint32_t b0, b1, b2, b3;   // ranks 8n .. 8n+7 (k low, k high), then 8n+8 .. (the last odd one twice)
-                        const int r = n + 1 < NT ? n * 8 + (lane & 7) + ((lane >> 4) << 3) : n * 8 + (lane & 7);
-                        ldsm_x4(tile_at(sa, r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
-                        mma_16816(acc[n], x0, x1, x2, x3, b0, b1);
-                        if (n + 1 < NT) mma_16816(acc[n + 1], x0, x1, x2, x3, b2, b3);
+                            for (int i = 0; i < 16; i++) v[i] += w[i];
+                        }
+                        uint32_t hi[8], low[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float v0 = mine == s ? v[2 * i] * sc : 0.f, v1 = mine == s ? v[2 * i + 1] * sc : 0.f;
+                            const __half2 h = __floats2half2_rn(v0, v1);
+                            const float2 f = __half22float2(h);
+                            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                            low[i] = pack_half2(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
+                        }
+                        if (!real) continue;
+                        uint4* o = reinterpret_cast<uint4*>(out + c);
+                        uint4* o2 = reinterpret_cast<uint4*>(out + part + c);
+                        o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if (p.parts == 2) o2[0] = make_uint4(low[0], low[1], low[2], low[3]);
+                        if (c + 16 <= rank) {
+                            o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                            if (p.parts == 2) o2[1] = make_uint4(low[4], low[5], low[6], low[7]);
+                        }
                     }
                 }
             }
-            cp_async_wait<0>();
+            tc_fence_before();
+            plan_sync();                      // the accumulators are read before the next pass's products
+            tc_fence_after();
         }
-        // masked, as fp16 (and what the rounding left, for fp32 outputs)
-        const float sc = a.scale ? a.scale[ad] : 1.f;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = local0 + warp * 16 + (lane >> 2) + 8 * h;
-            if (r >= n_rows) continue;
-            const bool on = row_adapter[r] == ad;
-            __half* out = p.t + ((first_block + s) * p.tile + r) * rank + (lane & 3) * 2;
-            const long long part = p.blocks * p.tile * rank;
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const float v0 = on ? acc[n][2 * h] * sc : 0.f, v1 = on ? acc[n][2 * h + 1] * sc : 0.f;
-                const __half2 hi = __floats2half2_rn(v0, v1);
-                *reinterpret_cast<__half2*>(out + n * 8) = hi;
-                if (p.parts == 2) {
-                    const float2 f = __half22float2(hi);
-                    const float l0 = isinf(f.x) ? 0.f : v0 - f.x, l1 = isinf(f.y) ? 0.f : v1 - f.y;
-                    *reinterpret_cast<__half2*>(out + part + n * 8) = __floats2half2_rn(l0, l1);
-                }
-            }
-        }
-        __syncthreads();       // the stages are read before the next adapter's copies
     }
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, shape.cols);
 }
 
-template <int NT>
-static int launch_nt(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
-    const int stages = stage_bytes(NT * 8) * 4 <= 64 * 1024 ? 4 : 3;
-    const int smem = stages * stage_bytes(NT * 8);
-    auto kern = lora_shrink_kernel<NT>;
+template <int ROWS>
+static int launch_rows(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
+    auto kern = lora_shrink_kernel<ROWS>;
     static bool attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!attr_set[dev & 63]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 218 * 1024) != cudaSuccess)
             return W2V_ERR_LAUNCH;
         attr_set[dev & 63] = true;
     }
-    // few row chunks: as many blocks per chunk as adapters can meet there, so that they run side by side
-    const long long chunks = (a.M + kRows - 1) / kRows;
+    CUtensorMap tx, ta;
+    const uint64_t xd[2] = {(uint64_t)a.K, (uint64_t)a.M}, xs[1] = {(uint64_t)a.lda * 2};
+    int rc = map_f16(&tx, a.x, 2, xd, xs, ROWS);
+    if (rc) return rc;
+    const uint64_t ad[3] = {(uint64_t)a.K, (uint64_t)p.rank, (uint64_t)a.n_adapters};
+    const uint64_t as[2] = {(uint64_t)a.K * 2, (uint64_t)a.K * 2 * p.rank};
+    rc = map_f16(&ta, a.a, 3, ad, as, p.rank);
+    if (rc) return rc;
+    // few row chunks: a block per two adapters that can meet there, side by side on the SMs
+    const long long chunks = (a.M + ROWS - 1) / ROWS;
     long long most = p.tile;
     if (a.n_utt < most) most = a.n_utt;
     if (a.n_adapters < most) most = a.n_adapters;
     long long ny = 296 / chunks;
-    ny = ny < 1 ? 1 : ny > most ? most : ny;
-    kern<<<dim3((unsigned)chunks, (unsigned)ny), kThreads, smem, st>>>(a, p, stages);
+    if (ny > (most + 1) / 2) ny = (most + 1) / 2;
+    if (ny < 1) ny = 1;
+    const ShrinkShape shape = shrink_shape(ROWS, p.rank);
+    kern<<<dim3((unsigned)chunks, (unsigned)ny), kThreads, shape.smem, st>>>(tx, ta, a, p, shape);
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
 
 int lora_shrink(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
-    switch (p.rank / 8) {
-#define W2V_SHRINK(n) case n: return launch_nt<n>(a, p, st);
-        W2V_SHRINK(1) W2V_SHRINK(2) W2V_SHRINK(3) W2V_SHRINK(4) W2V_SHRINK(5) W2V_SHRINK(6) W2V_SHRINK(7) W2V_SHRINK(8)
-        W2V_SHRINK(9) W2V_SHRINK(10) W2V_SHRINK(11) W2V_SHRINK(12) W2V_SHRINK(13) W2V_SHRINK(14) W2V_SHRINK(15) W2V_SHRINK(16)
-#undef W2V_SHRINK
-        default: return W2V_ERR_ARGS;
-    }
+    return p.tile % 128 == 0 && a.M >= 128 * 148 ? launch_rows<128>(a, p, st) : launch_rows<64>(a, p, st);
 }
 
 }  // namespace sg

@@ -17,8 +17,8 @@
 // zero in the other rows, and is multiplied by that adapter's B.  The delta
 // thus costs rank / K of the main product per adapter in the tile, is added
 // in fp32 before the only rounding, and needs no pass of its own over y.  The
-// kernel starts while the first product runs and waits for it only when a
-// tile's main K-blocks have been issued.
+// kernel starts while the first product runs and waits for it only before the
+// last K-block of its first tile.
 //
 // grouped: tiles are cut utterance by utterance (a warp-wide walk over the
 // utterances' lengths finds each tile, in order, so nothing is planned on the
@@ -39,6 +39,7 @@ constexpr int kSmemCap = 232448;
 constexpr int kABytes = kBM * kBK * 2;
 constexpr int kEpiBytes = kNE * 4096;          // per warp: a 32 x 32 fp32 chunk, or two fp16 store boxes
 constexpr int kMaxStages = 8;
+constexpr uint32_t kLastOfTile = 16;           // beside a stage's number of MMA steps
 
 struct Params {
     int M, N, k_blocks;
@@ -244,6 +245,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     uint64_t* tempty = tfull + 2;
     uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint32_t* stage_work = tmem_slot + 1;      // lora: what the MMA does with a stage
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -281,46 +283,53 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int chunks = LORA ? (p.plan.rank + kBK - 1) / kBK : 0;
 
     if (warp == 0) {
-        const uint32_t full_lead = PAIR ? mapa_shared(smem_u32(full), 0) : 0u;
+        // the leader's barriers count the bytes of a pair
+        const uint32_t lead = elect_one(), full_lead = PAIR ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+        const uint32_t arm = lead & (uint32_t)(rank == 0), base = smem_u32(smem), arm_bytes = (uint32_t)(CT * stage_bytes);
+        const int b_row = (int)rank * (p.bn / 2);
         int stage = 0;
         uint32_t phase = 0, issued = 0, last_par = 0;
-        bool ok = true, waited = !LORA;
+        bool ok = true;
+        // one stage's two tiles; work: its MMA steps, and whether it is the tile's last
+        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int k, int ra, int rb, int gb, uint32_t work) {
+            if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
+            const uint32_t dst = base + (uint32_t)(stage * stage_bytes), bar = full_lead + (uint32_t)(stage * 8);
+            if (LORA && lane == 0) stage_work[stage] = work;
+            if (LORA) __syncwarp();
+            expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
+            tma_load_2d_if<PAIR>(lead, dst, ma, bar, k, ra + (int)rank * kBM);
+            tma_load_3d_if<PAIR>(lead, dst + kABytes, mb, bar, k, rb + b_row, gb);
+            issued |= 1u << stage;
+            last_par = (last_par & ~(1u << stage)) | (phase << stage);
+            if (++stage == S) { stage = 0; phase ^= 1u; }
+        };
         for (int tile = unit; tile < total && ok; tile += n_units) {
             const Tile t = tile_at(tile);
-            if (lane == 0) {
-                auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int ka, int ra, int kb, int rb, int gb) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
-                    uint8_t* sa = smem + stage * stage_bytes;
-                    if constexpr (PAIR) {
-                        const uint32_t fb = full_lead + (uint32_t)(stage * 8);
-                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * stage_bytes);
-                        tma_load_2d_pair(sa, ma, fb, ka, ra + (int)rank * kBM);
-                        tma_load_4d_pair(sa + kABytes, mb, fb, kb, rb + (int)rank * (p.bn / 2), gb, 0);
-                    } else {
-                        mbar_arrive_expect_tx(&full[stage], stage_bytes);
-                        tma_load_2d(sa, ma, &full[stage], ka, ra);
-                        tma_load_4d(sa + kABytes, mb, &full[stage], kb, rb, gb, 0);
-                    }
-                    issued |= 1u << stage;
-                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
-                    if (++stage == S) { stage = 0; phase ^= 1u; }
-                };
-                for (int kb = 0; kb < p.k_blocks && ok; kb++)
-                    stage_in(&tmA, &tmB, kb * kBK, t.row0, kb * kBK, t.ni * p.bn, t.group);
-                if (LORA && p.lora) {
-                    if (!waited) { grid_dependency_wait(); waited = true; }
-                    const LoraTile lt = p.plan.tiles[t.row0 / kTileRows];
-                    for (int b = 0; b < lt.count && ok; b++) {
-                        const int ad = p.plan.adapter[lt.first + b];
-                        for (int part = 0; part < p.plan.parts; part++)
-                            for (int c = 0; c < chunks && ok; c++)
-                                stage_in(&tmT, &tmL, c * kBK,
-                                         (int)((part * p.plan.blocks + lt.first + b) * kTileRows), c * kBK,
-                                         t.ni * p.bn, ad);
+            const int col0 = t.ni * p.bn;
+            for (int kb = 0; kb < p.k_blocks - 1 && ok; kb++)
+                stage_in(&tmA, &tmB, kb * kBK, t.row0, col0, t.group, kBK / 16);
+            int blocks = 0, first = 0, rec = 0;
+            if (LORA && p.lora) {
+                if (tile == unit) grid_dependency_wait();
+                // the tile's record: first block, their number, the adapters of the first ones
+                rec = lane < 2 + kInline ? reinterpret_cast<const int*>(p.plan.tiles + t.row0 / kTileRows)[lane] : 0;
+                first = __shfl_sync(0xffffffffu, rec, 0);
+                blocks = __shfl_sync(0xffffffffu, rec, 1);
+            }
+            if (ok)
+                stage_in(&tmA, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile));
+            for (int b = 0; b < blocks && ok; b++) {
+                const int held = __shfl_sync(0xffffffffu, rec, min(2 + b, 31));
+                const int ad = b < kInline ? held : p.plan.adapter[first + b];
+                for (int part = 0; part < p.plan.parts; part++) {
+                    const int trow = (int)((part * p.plan.blocks + first + b) * kTileRows);
+                    for (int c = 0; c < chunks && ok; c++) {
+                        const bool last = b + 1 == blocks && part + 1 == p.plan.parts && c + 1 == chunks;
+                        stage_in(&tmT, &tmL, c * kBK, trow, col0, ad,
+                                 min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16) | (last ? kLastOfTile : 0));
                     }
                 }
             }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
         }
         // no bulk copy may still be writing shared memory when the CTA (or its peer) exits
         if (lane == 0 && rank == 0)
@@ -328,54 +337,40 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 if (issued & (1u << s)) mbar_wait(&full[s], (last_par >> s) & 1u, p.err);
         __syncwarp();
     } else if (warp == 1) {
-        if (rank == 0 && elect_one()) {
-            const uint32_t idesc = umma_idesc_f16(kTileRows, p.bn);
-            const uint32_t empty_peer = PAIR ? mapa_shared(smem_u32(empty), 1) : 0u;
-            const uint32_t tfull_peer = PAIR ? mapa_shared(smem_u32(tfull), 1) : 0u;
+        if (rank == 0) {
+            const uint32_t idesc = umma_idesc_f16(kTileRows, p.bn), lead = elect_one();
+            const uint64_t desc0 = umma_desc_sw128(smem_u32(smem));
+            const uint32_t empty_here = smem_u32(empty), empty_peer = PAIR ? mapa_shared(smem_u32(empty), 1) : 0u;
+            const uint32_t tfull_here = smem_u32(tfull), tfull_peer = PAIR ? mapa_shared(smem_u32(tfull), 1) : 0u;
             int stage = 0, it = 0;
             uint32_t phase = 0;
-            bool ok = true, waited = !LORA;
+            bool ok = true;
             for (int tile = unit; tile < total && ok; tile += n_units, it++) {
                 const int ab = it & 1;
-                if (!mbar_wait(&tempty[ab], ((uint32_t)(it >> 1) & 1u) ^ 1u, p.err)) break;
+                if (!mbar_wait_warp(&tempty[ab], ((uint32_t)(it >> 1) & 1u) ^ 1u, p.err)) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + (uint32_t)(ab * 256);
-                auto stage_mma = [&](bool first, int steps) {
-                    if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; return; }
+                for (int kb = 0; LORA || kb < p.k_blocks; kb++) {
+                    if (!mbar_wait_warp(&full[stage], phase, p.err)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + kABytes;
-                    for (int kk = 0; kk < steps; kk++) {
-                        const uint64_t da = umma_desc_sw128(a0 + kk * 32), db = umma_desc_sw128(b0 + kk * 32);
-                        if constexpr (PAIR) umma_f16_pair(d, da, db, idesc, !(first && kk == 0));
-                        else umma_f16(d, da, db, idesc, !(first && kk == 0));
-                    }
-                    if constexpr (PAIR) {
-                        umma_commit_pair(smem_u32(&empty[stage]));
-                        umma_commit_pair(empty_peer + (uint32_t)(stage * 8));
-                    } else {
-                        umma_commit(&empty[stage]);
-                    }
+                    const uint32_t work = LORA ? stage_work[stage] : kBK / 16;
+                    const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < kBK / 16; kk++)
+                        umma_f16_if<PAIR>(LORA ? lead & (uint32_t)(kk < (work & 15u)) : lead, d, desc_plus(da, kk * 32),
+                                          desc_plus(db, kk * 32), idesc, (kb | kk) != 0);
+                    umma_commit_if<PAIR>(lead, empty_here + (uint32_t)(stage * 8));
+                    if (PAIR) umma_commit_if<PAIR>(lead, empty_peer + (uint32_t)(stage * 8));
                     if (++stage == S) { stage = 0; phase ^= 1u; }
-                };
-                for (int kb = 0; kb < p.k_blocks && ok; kb++) stage_mma(kb == 0, kBK / 16);
-                if (LORA && p.lora && ok) {
-                    if (!waited) { grid_dependency_wait(); waited = true; }
-                    const int n = p.plan.tiles[tile / p.n_tiles].count * p.plan.parts;
-                    for (int b = 0; b < n; b++)
-                        for (int c = 0; c < chunks && ok; c++)
-                            stage_mma(false, min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16));
+                    if (LORA && (work & kLastOfTile)) break;
                 }
                 if (ok) {
-                    if constexpr (PAIR) {
-                        umma_commit_pair(smem_u32(&tfull[ab]));
-                        umma_commit_pair(tfull_peer + (uint32_t)(ab * 8));
-                    } else {
-                        umma_commit(&tfull[ab]);
-                    }
+                    umma_commit_if<PAIR>(lead, tfull_here + (uint32_t)(ab * 8));
+                    if (PAIR) umma_commit_if<PAIR>(lead, tfull_peer + (uint32_t)(ab * 8));
                 }
             }
             // no MMA may still be writing TMEM when it is freed (also after an expired wait)
-            if constexpr (PAIR) umma_commit_pair(smem_u32(done)); else umma_commit(done);
+            umma_commit_if<PAIR>(lead, smem_u32(done));
             mbar_wait(done, 0, p.err);
         }
         __syncwarp();
@@ -398,7 +393,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const bool box = kF16 && p.tma_c && (LORA ? row0 < t.end : row0 + 32 <= t.end);
             float4 res[8];
             if (EPI == W2V_EPI_F32_RESID && c0 < c1) load_resid(p, row0, t.end, col0 + c0 * 32, res);
-            if (!mbar_wait(&tfull[ab], (uint32_t)(it >> 1) & 1u, p.err)) break;
+            if (!mbar_wait_warp(&tfull[ab], (uint32_t)(it >> 1) & 1u, p.err)) break;
             tc_fence_after();
             const uint32_t trow = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * 256);
             if (kF16 && !box && nst) {          // boxes become the staging buffer
@@ -453,30 +448,6 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
-
-static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        cudaDriverEntryPointQueryResult q;
-        void* f = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-    }();
-    return fn;
-}
-
-// fp16 [.., rows, inner] with 64 x `box_rows` boxes, 128-byte swizzle.
-static int map_f16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, int box_rows) {
-    auto enc = get_encode();
-    if (!enc) return W2V_ERR_DRIVER;
-    const uint32_t box[4] = {kBK, (uint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
-    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims, strides, box, es,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? W2V_OK
-               : W2V_ERR_TENSOR_MAP;
-}
 
 struct Maps {
     CUtensorMap a, b, c, t, l;
@@ -537,7 +508,11 @@ static int launch_epi(int epi, const Maps& m, const Params& p, int tiles, bool d
     }
 }
 
-// Tile: width (a multiple of 32) and single CTAs or pairs, by waves x time per tile.
+// Tile: width w (a multiple of 32) and single CTAs or pairs, by waves over the
+// SMs x the cycles of a tile.  A K-block of 64 takes an SM 2 w cycles of MMA; its
+// operands, 16 KB of rows and 128 w bytes of weights (half of that in a pair, which
+// shares them), come in at some 64 bytes a cycle.  A wave also has a fill, a
+// drain and an epilogue.
 static void pick_tile(int N, long long m_tiles1, long long m_tiles2, long long K, int* bn, bool* pair) {
     double best = 1e300;
     for (int pr = 0; pr < 2; pr++)
@@ -546,7 +521,8 @@ static void pick_tile(int N, long long m_tiles1, long long m_tiles2, long long K
             const long long tiles = (pr ? m_tiles2 : m_tiles1) * ((N + w - 1) / w);
             const long long slots = pr ? 74 : 148;
             const long long waves = (tiles + slots - 1) / slots;
-            const double cost = (double)waves * (w * (pr ? 1.0 : 1.1) + 48) * (K + 400);
+            const double block = std::max(2.0 * w, 256.0 + (pr ? 1.0 : 2.0) * w);
+            const double cost = (double)waves * (K / kBK * block + 600 + 6.0 * w);
             if (cost < best) { best = cost; *bn = w; *pair = pr != 0; }
         }
 }
@@ -603,9 +579,9 @@ static int common(const Call& c, int bn, bool pair, Params& p, Maps& m) {
     const uint64_t ad[2] = {(uint64_t)c.K, (uint64_t)c.M}, as[1] = {(uint64_t)c.lda * 2};
     int rc = map_f16(&m.a, c.A, 2, ad, as, kBM);
     if (rc) return rc;
-    const uint64_t bd[4] = {(uint64_t)c.K, (uint64_t)c.N, (uint64_t)c.n_mats, 1};
-    const uint64_t bs[3] = {(uint64_t)c.K * 2, (uint64_t)c.K * 2 * c.N, (uint64_t)c.K * 2 * c.N * c.n_mats};
-    rc = map_f16(&m.b, c.B, 4, bd, bs, pair ? bn / 2 : bn);
+    const uint64_t bd[3] = {(uint64_t)c.K, (uint64_t)c.N, (uint64_t)c.n_mats};
+    const uint64_t bs[2] = {(uint64_t)c.K * 2, (uint64_t)c.K * 2 * c.N};
+    rc = map_f16(&m.b, c.B, 3, bd, bs, pair ? bn / 2 : bn);
     if (rc) return rc;
     m.c = m.t = m.l = m.a;
     // fp16 C by 32 x 32 boxes; a store clips the innermost dimension at 16-byte granularity only
@@ -662,9 +638,9 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
         const uint64_t ts[1] = {(uint64_t)rank * 2};
         rc = map_f16(&m.t, p.plan.t, 2, td, ts, kBM);
         if (rc) return rc;
-        const uint64_t ld[4] = {(uint64_t)rank, (uint64_t)N, (uint64_t)n_adapters, 1};
-        const uint64_t ls[3] = {(uint64_t)rank * 2, (uint64_t)rank * 2 * N, (uint64_t)rank * 2 * N * n_adapters};
-        rc = map_f16(&m.l, lora_b, 4, ld, ls, pair ? bn / 2 : bn);
+        const uint64_t ld[3] = {(uint64_t)rank, (uint64_t)N, (uint64_t)n_adapters};
+        const uint64_t ls[2] = {(uint64_t)rank * 2, (uint64_t)rank * 2 * N};
+        rc = map_f16(&m.l, lora_b, 3, ld, ls, pair ? bn / 2 : bn);
         if (rc) return rc;
         LoraArgs a;
         a.x = reinterpret_cast<const __half*>(A);
@@ -678,6 +654,7 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
         a.T = T;
         a.adapter = adapter;
         a.n_utt = n_utt;
+        a.err = err;
         rc = lora_shrink(a, p.plan, st);
         if (rc) return rc;
     }
@@ -698,9 +675,10 @@ extern "C" int w2v_gemm_grouped_f16(const void* A, long long lda, long long K, l
     Maps m;
     int bn = 256;
     bool pair = false;
-    // row tiles: at most one more than its rows need per utterance
-    const long long more = n_utt < M ? n_utt : M;
-    pick_tile(N, M / 128 + more, M / 256 + more, K, &bn, &pair);
+    // row tiles: as if the rows were spread evenly, and (below) at most one more than its rows
+    // need per utterance
+    const long long more = n_utt < M ? n_utt : M, mean = M / more;
+    pick_tile(N, more * ((mean + 127) / 128), more * ((mean + 255) / 256), K, &bn, &pair);
     int rc = common(c, bn, pair, p, m);
     if (rc) return rc;
     p.off = off;

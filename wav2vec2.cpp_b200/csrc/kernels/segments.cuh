@@ -2,19 +2,10 @@
 // and what the adapter kernels pass from the first product to the second.
 #pragma once
 #include "common.cuh"
+#include "w2v_kernels.h"
 
 namespace w2v {
 namespace sg {
-
-// The utterance that row r belongs to, or -1.
-W2V_DEV int utterance_of(const long long* off, const int* T, int n_utt, long long r) {
-    int lo = 0, hi = n_utt;      // first utterance that ends after r
-    while (lo < hi) {
-        const int m = (lo + hi) / 2;
-        if (off[m] + max(T[m], 0) > r) hi = m; else lo = m + 1;
-    }
-    return lo < n_utt && off[lo] <= r ? lo : -1;
-}
 
 // Low-rank adapters: s_a A_a x of every row, laid out for a GEMM whose tiles
 // take `tile` rows.  For each adapter that a tile's rows use there is a block
@@ -22,11 +13,13 @@ W2V_DEV int utterance_of(const long long* off, const int* T, int n_utt, long lon
 // second product is (block) x (that adapter's B): further K-blocks of the
 // tile's main product, however the tile's rows are spread over utterances.
 // Tile i's blocks are first .. first + count - 1 with
-//   first = i + min(utterances that start before the tile, rows before it),
-// which leaves room for every tile without a scan over the tiles before: a
-// tile has at most one utterance that started before it, and one per start in it.
-struct LoraTile {
+//   first = i + min(utterances that end before the tile, rows before it),
+// which leaves room for every tile without a scan over the tiles before: of a
+// tile's utterances all but one end in it.
+constexpr int kInline = 14;
+struct LoraTile {          // 64 bytes: one load of half a warp
     int first, count;
+    int adapter[kInline];  // of the first blocks; those of the others in LoraPlan::adapter
 };
 struct LoraPlan {
     LoraTile* tiles;       // [row tiles]
@@ -50,6 +43,7 @@ struct LoraArgs {
     const int* T;
     const int* adapter;
     int n_utt;
+    int* err;
 };
 
 __host__ inline long long lora_blocks(long long M, int n_utt, int tile) {
@@ -59,7 +53,7 @@ __host__ inline long long lora_blocks(long long M, int n_utt, int tile) {
 __host__ inline long long lora_workspace(long long M, int n_utt, int rank) {
     const long long rows = M + 256 * (1 + (n_utt < M ? n_utt : M));
     const long long tiles = M / 64 + 1;
-    return (tiles * 8 + 255) / 256 * 256 + ((tiles + (n_utt < M ? n_utt : M)) * 4 + 255) / 256 * 256 + rows * rank * 4 + 256;
+    return (tiles * (long long)sizeof(LoraTile) + 255) / 256 * 256 + ((tiles + (n_utt < M ? n_utt : M)) * 4 + 255) / 256 * 256 + rows * rank * 4 + 256;
 }
 __host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, int tile, int parts) {
     LoraPlan p;
@@ -69,7 +63,7 @@ __host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, i
     p.parts = parts;
     p.blocks = lora_blocks(M, n_utt, tile);
     p.tiles = reinterpret_cast<LoraTile*>(at);
-    at += ((M + tile - 1) / tile * 8 + 255) / 256 * 256;
+    at += ((M + tile - 1) / tile * (long long)sizeof(LoraTile) + 255) / 256 * 256;
     p.adapter = reinterpret_cast<int*>(at);
     at += (p.blocks * 4 + 255) / 256 * 256;
     p.t = reinterpret_cast<__half*>(at);
@@ -79,6 +73,117 @@ __host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, i
 // Fills the plan: lora_shrink.cu.  The launch lets the next kernel of the
 // stream start early; that one waits (grid_dependency_wait) before it reads the plan.
 int lora_shrink(const LoraArgs& a, const LoraPlan& p, cudaStream_t st);
+
+inline PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        cudaDriverEntryPointQueryResult q;
+        void* f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// fp16 [.., rows, inner] with 64 x `box_rows` boxes, 128-byte swizzle.
+inline int map_f16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, int box_rows) {
+    auto enc = get_encode();
+    if (!enc) return W2V_ERR_DRIVER;
+    const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims, strides, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? W2V_OK
+               : W2V_ERR_TENSOR_MAP;
+}
+
+// ── MMA issue from warp-uniform code ───────────────────────────────────────
+// The whole warp runs the issuing loop and one elected lane's predicate guards
+// the instructions: loop counters, descriptors and barriers then stay in
+// uniform registers.  Under a branch on the lane the operands of every MMA have
+// to be moved there first, some 200 cycles each, which bounds tiles of few columns.
+// The whole warp's wait, with one answer for all lanes.
+W2V_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+W2V_DEV uint64_t desc_plus(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
+template <bool PAIR>
+W2V_DEV void umma_f16_if(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                         uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+            : "memory");
+}
+// bar: shared::cluster address
+template <bool PAIR>
+W2V_DEV void umma_commit_if(uint32_t lead, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+            "r"(lead)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+            "r"(lead)
+            : "memory");
+}
+
+// TMA loads by the same scheme (some 450 cycles a stage of two loads otherwise).
+// bar: shared::cluster address of the barrier that counts the bytes.
+W2V_DEV void expect_tx_if(uint32_t lead, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+        " @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar),
+        "r"(bytes), "r"(lead)
+        : "memory");
+}
+template <bool PAIR>
+W2V_DEV void tma_load_2d_if(uint32_t lead, uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+            " @q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];\n}" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(lead)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+            " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];\n}" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(lead)
+            : "memory");
+}
+template <bool PAIR>
+W2V_DEV void tma_load_3d_if(uint32_t lead, uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"
+            " @q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];\n}" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(lead)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"
+            " @q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];\n}" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(lead)
+            : "memory");
+}
 
 W2V_DEV void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 W2V_DEV void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
