@@ -25,13 +25,9 @@ constexpr int kPlanners = 128, kThreads = kPlanners + 32;
 constexpr int kMaxRing = 8;
 
 struct ShrinkShape {
-    int stages, stage_bytes, smem;
-    int split, cols;       // accumulators of an adapter; columns of TMEM
+    int stages, stage_bytes, smem, cols;       // cols: of TMEM
 };
-// Two blocks per SM where a ring of three stages or more allows it.  An MMA of
-// few columns waits longer for the one before it on the same accumulator than it
-// takes (some 200 cycles at 16), so the MMAs of a stage go to up to four
-// accumulators in turn, which the epilogue adds: 64 x 10 s, K 768, rank 16 X us.
+// Two blocks per SM where a ring of three stages or more allows it.
 static ShrinkShape shrink_shape(int rows, int rank) {
     ShrinkShape s;
     s.stage_bytes = (rows + 2 * rank) * kStep * 2;
@@ -40,10 +36,8 @@ static ShrinkShape shrink_shape(int rows, int rank) {
     s.stages = two >= 3 ? two : one;
     if (s.stages > kMaxRing) s.stages = kMaxRing;
     s.smem = 1024 + s.stages * s.stage_bytes + behind + 256;
-    const int n16 = (rank + 15) / 16 * 16;
-    s.split = n16 <= 32 ? 4 : n16 <= 64 ? 2 : 1;
     s.cols = 32;
-    while (s.cols < 2 * s.split * n16) s.cols *= 2;
+    while (s.cols < 2 * ((rank + 15) / 16 * 16)) s.cols *= 2;
     return s;
 }
 
@@ -80,7 +74,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     __shared__ uint32_t tmem_slot;
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* ring = smem_raw + (((raw + 1023u) & ~1023u) - raw);
-    const int S = shape.stages, split = shape.split;
+    const int S = shape.stages;
     const int rank = p.rank, n16 = (rank + 15) / 16 * 16, a_bytes = rank * kStep * 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long row0 = (long long)blockIdx.x * kRows;
@@ -93,21 +87,23 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     // the block that is sure to use its rows fetches the first of them before it knows the adapters
     const int early = blockIdx.y == 0 ? min(S, k_steps) : 0;
 
-    // a stage's x (and the adapters' share) arrives on full[st]: two arrivals
+    // a stage's x and the adapters' share complete on full[st]
     const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), lead = elect_one();
     auto load_x = [&](int st, int ks) {
-        expect_tx_if(lead, full0 + (uint32_t)(st * 8), kXBytes);
         tma_load_2d_if<false>(lead, ring0 + (uint32_t)(st * shape.stage_bytes), &tmX, full0 + (uint32_t)(st * 8), ks * kStep,
                               (int)row0);
     };
     if (warp == kPlanners / 32) {
         if (lane == 0) {
-            for (int s = 0; s < S; s++) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
+            for (int s = 0; s < S; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
             mbar_init(&done, 1);
             fence_mbar_init();
         }
         __syncwarp();
-        for (int ks = 0; ks < early; ks++) load_x(ks, ks);
+        for (int ks = 0; ks < early; ks++) {
+            expect_more_if(lead, full0 + (uint32_t)(ks * 8), kXBytes);
+            load_x(ks, ks);
+        }
     }
     if (warp == 0) {
         // TMEM first: a projection's block that came to this SM before would hold all of it
@@ -283,23 +279,23 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const int n_here = n_here_shared;
     const long long first_block = first_block_shared;
 
-    // two adapters a pass; the ring's counters run on
-    const uint32_t tmem = tmem_slot;
+    // adapters of a pass: two, or one where there are blocks for each; the ring's counters run on
+    const int side = n_here > (int)gridDim.y ? 2 : 1;
+    const uint32_t tmem = (uint32_t)uniform((int)tmem_slot);
     if (warp == kPlanners / 32) {
         int st = 0, used = 0;                 // used: stages filled so far
         uint32_t odd = 0, issued = 0;
         bool ok = true;
-        for (int base = 2 * blockIdx.y; base < n_here && ok; base += 2 * gridDim.y) {
-            const int n = min(2, n_here - base);
-            const int ad0 = slots[here[base]], ad1 = n > 1 ? slots[here[base + 1]] : 0;
-            const uint32_t second = n > 1 ? lead : 0u;
+        for (int base = side * blockIdx.y; base < n_here && ok; base += side * gridDim.y) {
+            const int n = uniform(min(side, n_here - base));
+            const int ad0 = uniform(slots[here[base]]), ad1 = uniform(n > 1 ? slots[here[base + 1]] : 0);
             for (int ks = 0; ks < k_steps; ks++) {
                 if (used >= S && !mbar_wait_warp(&empty[st], odd ^ 1u, a.err)) { ok = false; break; }
-                if (used >= early) load_x(st, ks);
                 const uint32_t sa = ring0 + (uint32_t)(st * shape.stage_bytes + kXBytes), bar = full0 + (uint32_t)(st * 8);
-                expect_tx_if(lead, bar, (uint32_t)(n * a_bytes));
+                expect_tx_if(lead, bar, (uint32_t)(n * a_bytes + (used >= early ? kXBytes : 0)));
                 tma_load_3d_if<false>(lead, sa, &tmA, bar, ks * kStep, 0, ad0);
-                tma_load_3d_if<false>(second, sa + (uint32_t)a_bytes, &tmA, bar, ks * kStep, 0, ad1);
+                if (n > 1) tma_load_3d_if<false>(lead, sa + (uint32_t)a_bytes, &tmA, bar, ks * kStep, 0, ad1);
+                if (used >= early) load_x(st, ks);
                 issued |= 1u << st;
                 used++;
                 if (++st == S) { st = 0; odd ^= 1u; }
@@ -318,8 +314,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         int st = 0, pass = 0;
         uint32_t odd = 0;
         bool ok = true;
-        for (int base = 2 * blockIdx.y; base < n_here; base += 2 * gridDim.y, pass++) {
-            const int n = min(2, n_here - base);
+        for (int base = side * blockIdx.y; base < n_here; base += side * gridDim.y, pass++) {
+            const int n = min(side, n_here - base);
             if (warp == 0) {
                 const uint32_t idesc = umma_idesc_f16(128, n16);
                 const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
@@ -329,11 +325,11 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     const uint64_t dx = desc_plus(desc0, (uint32_t)(st * shape.stage_bytes));
                     for (int e = 0; e < n; e++) {
                         const uint64_t db = desc_plus(dx, (uint32_t)(kXBytes + e * a_bytes));
-                        const uint32_t d = tmem + (uint32_t)(e * split * n16);
+                        const uint32_t d = tmem + (uint32_t)(e * n16);
 #pragma unroll
                         for (int kk = 0; kk < kStep / 16; kk++)
-                            umma_f16_if<false>(lead, d + (uint32_t)((kk & (split - 1)) * n16), desc_plus(dx, kk * 32),
-                                               desc_plus(db, kk * 32), idesc, ks != 0 || kk >= split);
+                            umma_f16_if<false>(lead, d, desc_plus(dx, kk * 32), desc_plus(db, kk * 32), idesc,
+                                               (ks | kk) != 0);
                     }
                     umma_commit_if<false>(lead, smem_u32(&empty[st]));
                     if (++st == S) { st = 0; odd ^= 1u; }
@@ -353,14 +349,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * rank;
                     for (int c = 0; c < rank; c += 16) {
                         float v[16];
-                        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * split * n16 + c);
-                        tmem_ld16(at, v);
-                        for (int q = 1; q < split; q++) {
-                            float w[16];
-                            tmem_ld16(at + (uint32_t)(q * n16), w);
-#pragma unroll
-                            for (int i = 0; i < 16; i++) v[i] += w[i];
-                        }
+                        tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * n16 + c), v);
                         uint32_t hi[8], low[8];
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
@@ -410,13 +399,13 @@ static int launch_rows(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
     const uint64_t as[2] = {(uint64_t)a.K * 2, (uint64_t)a.K * 2 * p.rank};
     rc = map_f16(&ta, a.a, 3, ad, as, p.rank);
     if (rc) return rc;
-    // few row chunks: a block per two adapters that can meet there, side by side on the SMs
+    // few row chunks: a block per adapter that can meet there, side by side on the SMs
     const long long chunks = (a.M + ROWS - 1) / ROWS;
     long long most = p.tile;
     if (a.n_utt < most) most = a.n_utt;
     if (a.n_adapters < most) most = a.n_adapters;
     long long ny = 296 / chunks;
-    if (ny > (most + 1) / 2) ny = (most + 1) / 2;
+    if (ny > most) ny = most;
     if (ny < 1) ny = 1;
     const ShrinkShape shape = shrink_shape(ROWS, p.rank);
     kern<<<dim3((unsigned)chunks, (unsigned)ny), kThreads, shape.smem, st>>>(tx, ta, a, p, shape);

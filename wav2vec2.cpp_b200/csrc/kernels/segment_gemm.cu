@@ -117,9 +117,9 @@ struct Walker {
         const int src = __ffs(past) - 1;
         const int prev = __shfl_sync(0xffffffffu, incl, src > 0 ? src - 1 : 0);
         const int k = m - before - (src > 0 ? prev : 0);
-        t.row0 = __shfl_sync(0xffffffffu, first, src) + k * tile_rows;
-        t.end = __shfl_sync(0xffffffffu, end, src);
-        t.group = __shfl_sync(0xffffffffu, group, src);
+        t.row0 = uniform(__shfl_sync(0xffffffffu, first, src) + k * tile_rows);
+        t.end = uniform(__shfl_sync(0xffffffffu, end, src));
+        t.group = uniform(__shfl_sync(0xffffffffu, group, src));
     }
 };
 
@@ -231,7 +231,8 @@ template <int EPI, bool PAIR, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1)
 seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmT,
-                const __grid_constant__ CUtensorMap tmL, const __grid_constant__ Params p) {
+                const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmA32,
+                const __grid_constant__ CUtensorMap tmT32, const __grid_constant__ Params p) {
     constexpr int CT = PAIR ? 2 : 1, kTileRows = kBM * CT;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
@@ -267,7 +268,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     tc_fence_before();
     if (PAIR) cluster_sync_all(); else __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = (uint32_t)uniform((int)*tmem_slot);
 
     Walker walk;
     const int total = (LORA ? p.m_tiles : walk.count(p, kTileRows)) * p.n_tiles;
@@ -285,19 +286,29 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     if (warp == 0) {
         // the leader's barriers count the bytes of a pair
         const uint32_t lead = elect_one(), full_lead = PAIR ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
-        const uint32_t arm = lead & (uint32_t)(rank == 0), base = smem_u32(smem), arm_bytes = (uint32_t)(CT * stage_bytes);
+        const uint32_t arm = lead & (uint32_t)(rank == 0), base = smem_u32(smem);
+        uint32_t arm_bytes = 0;                // of a stage, both CTAs' in a pair
         const int b_row = (int)rank * (p.bn / 2);
         int stage = 0;
         uint32_t phase = 0, issued = 0, last_par = 0;
         bool ok = true;
         // one stage's two tiles; work: its MMA steps, and whether it is the tile's last
-        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int k, int ra, int rb, int gb, uint32_t work) {
+        // of the rows only the 32-row boxes that hold valid ones, where that saves any: what the MMA
+        // reads in the others' places goes to accumulator rows that are not stored
+        int boxes = 4;
+        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* ma32, const CUtensorMap* mb, int k, int ra, int rb, int gb,
+                            uint32_t work) {
             if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
             const uint32_t dst = base + (uint32_t)(stage * stage_bytes), bar = full_lead + (uint32_t)(stage * 8);
             if (LORA && lane == 0) stage_work[stage] = work;
             if (LORA) __syncwarp();
             expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
-            tma_load_2d_if<PAIR>(lead, dst, ma, bar, k, ra + (int)rank * kBM);
+            if (boxes == 4) {
+                tma_load_2d_if<PAIR>(lead, dst, ma, bar, k, ra + (int)rank * kBM);
+            } else {
+                for (int i = 0; i < boxes; i++)
+                    tma_load_2d_if<PAIR>(lead, dst + (uint32_t)(i * kABytes / 4), ma32, bar, k, ra + (int)rank * kBM + i * 32);
+            }
             tma_load_3d_if<PAIR>(lead, dst + kABytes, mb, bar, k, rb + b_row, gb);
             issued |= 1u << stage;
             last_par = (last_par & ~(1u << stage)) | (phase << stage);
@@ -306,26 +317,29 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         for (int tile = unit; tile < total && ok; tile += n_units) {
             const Tile t = tile_at(tile);
             const int col0 = t.ni * p.bn;
+            auto boxes_of = [&](int r) { return max(min((t.end - r + 31) / 32, 4), 0); };
+            boxes = boxes_of(t.row0 + (int)rank * kBM);
+            arm_bytes = (uint32_t)(CT * p.b_bytes + (boxes_of(t.row0) + (PAIR ? boxes_of(t.row0 + kBM) : 0)) * (kABytes / 4));
             for (int kb = 0; kb < p.k_blocks - 1 && ok; kb++)
-                stage_in(&tmA, &tmB, kb * kBK, t.row0, col0, t.group, kBK / 16);
+                stage_in(&tmA, &tmA32, &tmB, kb * kBK, t.row0, col0, t.group, kBK / 16);
             int blocks = 0, first = 0, rec = 0;
             if (LORA && p.lora) {
                 if (tile == unit) grid_dependency_wait();
                 // the tile's record: first block, their number, the adapters of the first ones
                 rec = lane < 2 + kInline ? reinterpret_cast<const int*>(p.plan.tiles + t.row0 / kTileRows)[lane] : 0;
-                first = __shfl_sync(0xffffffffu, rec, 0);
-                blocks = __shfl_sync(0xffffffffu, rec, 1);
+                first = uniform(__shfl_sync(0xffffffffu, rec, 0));
+                blocks = uniform(__shfl_sync(0xffffffffu, rec, 1));
             }
             if (ok)
-                stage_in(&tmA, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile));
+                stage_in(&tmA, &tmA32, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile));
             for (int b = 0; b < blocks && ok; b++) {
                 const int held = __shfl_sync(0xffffffffu, rec, min(2 + b, 31));
-                const int ad = b < kInline ? held : p.plan.adapter[first + b];
+                const int ad = uniform(b < kInline ? held : p.plan.adapter[first + b]);
                 for (int part = 0; part < p.plan.parts; part++) {
                     const int trow = (int)((part * p.plan.blocks + first + b) * kTileRows);
                     for (int c = 0; c < chunks && ok; c++) {
                         const bool last = b + 1 == blocks && part + 1 == p.plan.parts && c + 1 == chunks;
-                        stage_in(&tmT, &tmL, c * kBK, trow, col0, ad,
+                        stage_in(&tmT, &tmT32, &tmL, c * kBK, trow, col0, ad,
                                  min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16) | (last ? kLastOfTile : 0));
                     }
                 }
@@ -353,7 +367,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 for (int kb = 0; LORA || kb < p.k_blocks; kb++) {
                     if (!mbar_wait_warp(&full[stage], phase, p.err)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t work = LORA ? stage_work[stage] : kBK / 16;
+                    const uint32_t work = LORA ? (uint32_t)uniform((int)stage_work[stage]) : kBK / 16;
                     const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
 #pragma unroll
                     for (uint32_t kk = 0; kk < kBK / 16; kk++)
@@ -450,7 +464,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 // ── host side ───────────────────────────────────────────────────────────────
 
 struct Maps {
-    CUtensorMap a, b, c, t, l;
+    CUtensorMap a, b, c, t, l, a32, t32;
 };
 
 template <int EPI, bool PAIR, bool LORA>
@@ -494,7 +508,7 @@ static int launch(const Maps& m, const Params& p, int tiles, bool dependent, cud
         attr[n].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = ++n;
     }
-    if (cudaLaunchKernelEx(&cfg, kern, m.a, m.b, m.c, m.t, m.l, p) != cudaSuccess) return W2V_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kern, m.a, m.b, m.c, m.t, m.l, m.a32, m.t32, p) != cudaSuccess) return W2V_ERR_LAUNCH;
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
 
@@ -578,12 +592,13 @@ static int common(const Call& c, int bn, bool pair, Params& p, Maps& m) {
     p.err = c.err;
     const uint64_t ad[2] = {(uint64_t)c.K, (uint64_t)c.M}, as[1] = {(uint64_t)c.lda * 2};
     int rc = map_f16(&m.a, c.A, 2, ad, as, kBM);
+    if (!rc) rc = map_f16(&m.a32, c.A, 2, ad, as, 32);
     if (rc) return rc;
     const uint64_t bd[3] = {(uint64_t)c.K, (uint64_t)c.N, (uint64_t)c.n_mats};
     const uint64_t bs[2] = {(uint64_t)c.K * 2, (uint64_t)c.K * 2 * c.N};
     rc = map_f16(&m.b, c.B, 3, bd, bs, pair ? bn / 2 : bn);
     if (rc) return rc;
-    m.c = m.t = m.l = m.a;
+    m.c = m.t = m.l = m.t32 = m.a;
     // fp16 C by 32 x 32 boxes; a store clips the innermost dimension at 16-byte granularity only
     p.tma_c = f16 && c.ldc % 8 == 0 && c.N % 8 == 0 && C % 16 == 0;
     if (p.tma_c) {
@@ -637,6 +652,7 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
         const uint64_t td[2] = {(uint64_t)rank, (uint64_t)(p.plan.parts * p.plan.blocks * tile_rows)};
         const uint64_t ts[1] = {(uint64_t)rank * 2};
         rc = map_f16(&m.t, p.plan.t, 2, td, ts, kBM);
+        if (!rc) rc = map_f16(&m.t32, p.plan.t, 2, td, ts, 32);
         if (rc) return rc;
         const uint64_t ld[3] = {(uint64_t)rank, (uint64_t)N, (uint64_t)n_adapters};
         const uint64_t ls[2] = {(uint64_t)rank * 2, (uint64_t)rank * 2 * N};

@@ -107,6 +107,9 @@ inline int map_f16(CUtensorMap* m, const void* base, int rank, const uint64_t* d
 W2V_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
+// A value that all lanes hold, in a uniform register (the operands of a TMA load
+// have to be there, and a value that came by a shuffle or from memory is not known to be).
+W2V_DEV int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 W2V_DEV uint64_t desc_plus(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 template <bool PAIR>
 W2V_DEV void umma_f16_if(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -147,6 +150,14 @@ W2V_DEV void expect_tx_if(uint32_t lead, uint32_t bar, uint32_t bytes) {
     asm volatile(
         "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
         " @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar),
+        "r"(bytes), "r"(lead)
+        : "memory");
+}
+// Bytes to come in the current phase, without an arrival.
+W2V_DEV void expect_more_if(uint32_t lead, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+        " @q mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n}" ::"r"(bar),
         "r"(bytes), "r"(lead)
         : "memory");
 }
