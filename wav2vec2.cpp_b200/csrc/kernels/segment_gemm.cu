@@ -20,6 +20,15 @@
 // kernel starts while the first product runs and waits for it only before the
 // last K-block of its first tile.
 //
+// fp32 outputs: the tensor core's accumulation drops what lies behind the 24th bit
+// of each partial sum, always towards zero, which over K = 1024 adds up to 1.2e-6 of
+// the result.  For them an accumulator is handed over every 512 of K (beside a residual:
+// 1024), the epilogue warps add it, rounding to nearest, to a running total that has
+// columns of its own in TMEM, and the error stays near that of an fp32 product (6e-7
+// at any K).  The
+// MMAs wait for the hand-over where the tile leaves no room for a second
+// accumulator (more than 160 columns).
+//
 // grouped: tiles are cut utterance by utterance (a warp-wide walk over the
 // utterances' lengths finds each tile, in order, so nothing is planned on the
 // host and no workspace is needed); rows past the utterance are computed and
@@ -39,7 +48,10 @@ constexpr int kSmemCap = 232448;
 constexpr int kABytes = kBM * kBK * 2;
 constexpr int kEpiBytes = kNE * 4096;          // per warp: a 32 x 32 fp32 chunk, or two fp16 store boxes
 constexpr int kMaxStages = 8;
-constexpr uint32_t kLastOfTile = 16;           // beside a stage's number of MMA steps
+constexpr uint32_t kLastOfTile = 16, kLastOfSum = 32;   // beside a stage's number of MMA steps
+__host__ __device__ constexpr bool sums_of(int epi) { return epi == W2V_EPI_F32 || epi == W2V_EPI_F32_RESID; }
+// K-blocks of a sum: 512 of K; beside a residual, which as a rule is larger than what is added to it, 1024.
+__host__ __device__ constexpr int sum_blocks(int epi) { return epi == W2V_EPI_F32_RESID ? 16 : 8; }
 
 struct Params {
     int M, N, k_blocks;
@@ -152,13 +164,14 @@ W2V_DEV void store_chunk(const Params& p, const float* stg, const float* bias, i
     const int col = col0 + 4 * cg;
     if (col >= p.N) return;
     const int n = min(4, p.N - col);
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
     if (bias) {
-        if (p.bias_vec && n == 4) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(bias + col));
-            b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
-        } else {
-            for (int j = 0; j < n; j++) b[j] = __ldg(bias + col + j);
+        if (p.bias_vec && n == 4) b = __ldg(reinterpret_cast<const float4*>(bias + col));
+        else {
+            b.x = __ldg(bias + col);
+            if (n > 1) b.y = __ldg(bias + col + 1);
+            if (n > 2) b.z = __ldg(bias + col + 2);
+            if (n > 3) b.w = __ldg(bias + col + 3);
         }
     }
     float4 xs[8];
@@ -168,21 +181,29 @@ W2V_DEV void store_chunk(const Params& p, const float* stg, const float* bias, i
     for (int i = 0; i < 8; i++) {
         const int r = row0 + rs + 4 * i;
         if (r >= end) continue;
-        float x[4] = {xs[i].x + b[0], xs[i].y + b[1], xs[i].z + b[2], xs[i].w + b[3]};
-        if (EPI == W2V_EPI_F32_RESID) { x[0] += res[i].x; x[1] += res[i].y; x[2] += res[i].z; x[3] += res[i].w; }
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = epi_value(EPI, x[j]);
+        float4 x = xs[i];
+        x.x += b.x; x.y += b.y; x.z += b.z; x.w += b.w;
+        if (EPI == W2V_EPI_F32_RESID) { x.x += res[i].x; x.y += res[i].y; x.z += res[i].z; x.w += res[i].w; }
+        x.x = epi_value(EPI, x.x); x.y = epi_value(EPI, x.y); x.z = epi_value(EPI, x.z); x.w = epi_value(EPI, x.w);
         const long long at = (long long)r * p.ldc + col;
         if (EPI == W2V_EPI_F16 || EPI == W2V_EPI_F16_GELU) {
             __half* c = reinterpret_cast<__half*>(p.C) + at;
-            if (p.vec && n == 4) *reinterpret_cast<uint2*>(c) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
-            else
-                for (int j = 0; j < n; j++) c[j] = __float2half_rn(x[j]);
+            if (p.vec && n == 4) *reinterpret_cast<uint2*>(c) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+            else {
+                c[0] = __float2half_rn(x.x);
+                if (n > 1) c[1] = __float2half_rn(x.y);
+                if (n > 2) c[2] = __float2half_rn(x.z);
+                if (n > 3) c[3] = __float2half_rn(x.w);
+            }
         } else {
             float* c = reinterpret_cast<float*>(p.C) + at;
-            if (p.vec && n == 4) *reinterpret_cast<float4*>(c) = make_float4(x[0], x[1], x[2], x[3]);
-            else
-                for (int j = 0; j < n; j++) c[j] = x[j];
+            if (p.vec && n == 4) *reinterpret_cast<float4*>(c) = x;
+            else {
+                c[0] = x.x;
+                if (n > 1) c[1] = x.y;
+                if (n > 2) c[2] = x.z;
+                if (n > 3) c[3] = x.w;
+            }
         }
     }
 }
@@ -227,6 +248,27 @@ W2V_DEV void store_box(const Params& p, const CUtensorMap* tmC, float (&v)[32], 
     }
 }
 
+// Two 32 x 32 blocks of TMEM (32 lanes, 32 columns) with one wait.
+W2V_DEV void tmem_ld32x2(uint32_t addr_a, float (&a)[32], uint32_t addr_b, float (&b)[32]) {
+    uint32_t r[32], s[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n"
+        " tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n"
+        " tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(s[0]), "=r"(s[1]), "=r"(s[2]), "=r"(s[3]), "=r"(s[4]), "=r"(s[5]), "=r"(s[6]), "=r"(s[7]),
+          "=r"(s[8]), "=r"(s[9]), "=r"(s[10]), "=r"(s[11]), "=r"(s[12]), "=r"(s[13]), "=r"(s[14]), "=r"(s[15]),
+          "=r"(s[16]), "=r"(s[17]), "=r"(s[18]), "=r"(s[19]), "=r"(s[20]), "=r"(s[21]), "=r"(s[22]), "=r"(s[23]),
+          "=r"(s[24]), "=r"(s[25]), "=r"(s[26]), "=r"(s[27]), "=r"(s[28]), "=r"(s[29]), "=r"(s[30]), "=r"(s[31])
+        : "r"(addr_a), "r"(addr_b)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) { a[i] = __uint_as_float(r[i]); b[i] = __uint_as_float(s[i]); }
+}
+
 template <int EPI, bool PAIR, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1)
 seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -234,6 +276,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmA32,
                 const __grid_constant__ CUtensorMap tmT32, const __grid_constant__ Params p) {
     constexpr int CT = PAIR ? 2 : 1, kTileRows = kBM * CT;
+    constexpr bool SUMS = sums_of(EPI), WORK = LORA || SUMS;   // WORK: a stage says what is to be done with it
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     // identical offset in both CTAs of a pair: the MMA addresses the peer's operands at the leader's offsets
@@ -246,7 +289,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     uint64_t* tempty = tfull + 2;
     uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-    uint32_t* stage_work = tmem_slot + 1;      // lora: what the MMA does with a stage
+    uint32_t* stage_work = tmem_slot + 1;      // what the MMA does with a stage
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -270,6 +313,12 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem_base = (uint32_t)uniform((int)*tmem_slot);
 
+    // accumulators: two, or with running totals (columns 0 .. bn - 1) one or two behind them
+    const int n_sums = SUMS ? (p.k_blocks + sum_blocks(EPI) - 1) / sum_blocks(EPI) : 1;
+    const uint32_t n_acc = n_sums > 1 && 3 * p.bn > 512 ? 1u : 2u;
+    auto accumulator_at = [&](uint32_t i) {
+        return tmem_base + (n_sums > 1 ? (uint32_t)p.bn * (1u + i) : i * 256u);
+    };
     Walker walk;
     const int total = (LORA ? p.m_tiles : walk.count(p, kTileRows)) * p.n_tiles;
     auto tile_at = [&](int tile) {
@@ -292,7 +341,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         int stage = 0;
         uint32_t phase = 0, issued = 0, last_par = 0;
         bool ok = true;
-        // one stage's two tiles; work: its MMA steps, and whether it is the tile's last
+        // one stage's two tiles; work: its MMA steps, and whether it is the last of a sum and of the tile
         // of the rows only the 32-row boxes that hold valid ones, where that saves any: what the MMA
         // reads in the others' places goes to accumulator rows that are not stored
         int boxes = 4;
@@ -300,8 +349,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             uint32_t work) {
             if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
             const uint32_t dst = base + (uint32_t)(stage * stage_bytes), bar = full_lead + (uint32_t)(stage * 8);
-            if (LORA && lane == 0) stage_work[stage] = work;
-            if (LORA) __syncwarp();
+            if (WORK && lane == 0) stage_work[stage] = work;
+            if (WORK) __syncwarp();
             expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
             if (boxes == 4) {
                 tma_load_2d_if<PAIR>(lead, dst, ma, bar, k, ra + (int)rank * kBM);
@@ -321,7 +370,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             boxes = boxes_of(t.row0 + (int)rank * kBM);
             arm_bytes = (uint32_t)(CT * p.b_bytes + (boxes_of(t.row0) + (PAIR ? boxes_of(t.row0 + kBM) : 0)) * (kABytes / 4));
             for (int kb = 0; kb < p.k_blocks - 1 && ok; kb++)
-                stage_in(&tmA, &tmA32, &tmB, kb * kBK, t.row0, col0, t.group, kBK / 16);
+                stage_in(&tmA, &tmA32, &tmB, kb * kBK, t.row0, col0, t.group,
+                         kBK / 16 | (SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1 ? kLastOfSum : 0));
             int blocks = 0, first = 0, rec = 0;
             if (LORA && p.lora) {
                 if (tile == unit) grid_dependency_wait();
@@ -331,7 +381,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 blocks = uniform(__shfl_sync(0xffffffffu, rec, 1));
             }
             if (ok)
-                stage_in(&tmA, &tmA32, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile));
+                stage_in(&tmA, &tmA32, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile | kLastOfSum));
             for (int b = 0; b < blocks && ok; b++) {
                 const int held = __shfl_sync(0xffffffffu, rec, min(2 + b, 31));
                 const int ad = uniform(b < kInline ? held : p.plan.adapter[first + b]);
@@ -340,7 +390,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     for (int c = 0; c < chunks && ok; c++) {
                         const bool last = b + 1 == blocks && part + 1 == p.plan.parts && c + 1 == chunks;
                         stage_in(&tmT, &tmT32, &tmL, c * kBK, trow, col0, ad,
-                                 min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16) | (last ? kLastOfTile : 0));
+                                 min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16) | (last ? kLastOfTile | kLastOfSum : 0));
                     }
                 }
             }
@@ -356,31 +406,36 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const uint64_t desc0 = umma_desc_sw128(smem_u32(smem));
             const uint32_t empty_here = smem_u32(empty), empty_peer = PAIR ? mapa_shared(smem_u32(empty), 1) : 0u;
             const uint32_t tfull_here = smem_u32(tfull), tfull_peer = PAIR ? mapa_shared(smem_u32(tfull), 1) : 0u;
-            int stage = 0, it = 0;
-            uint32_t phase = 0;
+            int stage = 0;
+            uint32_t phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
-            for (int tile = unit; tile < total && ok; tile += n_units, it++) {
-                const int ab = it & 1;
-                if (!mbar_wait_warp(&tempty[ab], ((uint32_t)(it >> 1) & 1u) ^ 1u, p.err)) break;
-                tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(ab * 256);
-                for (int kb = 0; LORA || kb < p.k_blocks; kb++) {
+            for (int tile = unit; tile < total && ok; tile += n_units) {
+                bool first = true;               // stage of a sum
+                uint32_t d = 0;
+                for (int kb = 0; WORK || kb < p.k_blocks; kb++) {
+                    if (first) {
+                        if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1u, p.err)) { ok = false; break; }
+                        d = accumulator_at(acc);
+                    }
                     if (!mbar_wait_warp(&full[stage], phase, p.err)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t work = LORA ? (uint32_t)uniform((int)stage_work[stage]) : kBK / 16;
+                    const uint32_t work = WORK ? (uint32_t)uniform((int)stage_work[stage])
+                                               : kBK / 16 | (kb == p.k_blocks - 1 ? kLastOfSum : 0);
                     const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
 #pragma unroll
                     for (uint32_t kk = 0; kk < kBK / 16; kk++)
                         umma_f16_if<PAIR>(LORA ? lead & (uint32_t)(kk < (work & 15u)) : lead, d, desc_plus(da, kk * 32),
-                                          desc_plus(db, kk * 32), idesc, (kb | kk) != 0);
+                                          desc_plus(db, kk * 32), idesc, !first || kk != 0);
                     umma_commit_if<PAIR>(lead, empty_here + (uint32_t)(stage * 8));
                     if (PAIR) umma_commit_if<PAIR>(lead, empty_peer + (uint32_t)(stage * 8));
                     if (++stage == S) { stage = 0; phase ^= 1u; }
-                    if (LORA && (work & kLastOfTile)) break;
-                }
-                if (ok) {
-                    umma_commit_if<PAIR>(lead, tfull_here + (uint32_t)(ab * 8));
-                    if (PAIR) umma_commit_if<PAIR>(lead, tfull_peer + (uint32_t)(ab * 8));
+                    first = (work & kLastOfSum) != 0;
+                    if (first) {
+                        umma_commit_if<PAIR>(lead, tfull_here + acc * 8u);
+                        if (PAIR) umma_commit_if<PAIR>(lead, tfull_peer + acc * 8u);
+                        if (++acc == n_acc) { acc = 0; acc_phase ^= 1u; }
+                    }
+                    if (WORK && (work & kLastOfTile)) break;
                 }
             }
             // no MMA may still be writing TMEM when it is freed (also after an expired wait)
@@ -395,22 +450,48 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const uint32_t tempty_lead = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0u;
         float* stg = reinterpret_cast<float*>(epi + (warp - 2) * 4096);
         constexpr bool kF16 = EPI == W2V_EPI_F16 || EPI == W2V_EPI_F16_GELU;
-        uint32_t nst = 0;
-        int it = 0;
-        for (int tile = unit; tile < total; tile += n_units, it++) {
+        uint32_t nst = 0, acc = 0, acc_phase = 0;
+        for (int tile = unit; tile < total; tile += n_units) {
             const Tile t = tile_at(tile);
-            const int ab = it & 1;
             const int row0 = t.row0 + (int)rank * kBM + q * 32;
             const int col0 = t.ni * p.bn;
             const float* bias = p.bias ? p.bias + (long long)t.group * p.bias_stride : nullptr;
             // whole boxes inside the rows to be written (lora: the map clips at M)
             const bool box = kF16 && p.tma_c && (LORA ? row0 < t.end : row0 + 32 <= t.end);
+            const uint32_t lanes = (uint32_t)(q * 32) << 16;
+            auto release = [&]() {               // hands the accumulator back
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_remote(tempty_lead + acc * 8u);
+                    else mbar_arrive(&tempty[acc]);
+                }
+                if (++acc == n_acc) { acc = 0; acc_phase ^= 1u; }
+            };
             float4 res[8];
             if (EPI == W2V_EPI_F32_RESID && c0 < c1) load_resid(p, row0, t.end, col0 + c0 * 32, res);
-            if (!mbar_wait_warp(&tfull[ab], (uint32_t)(it >> 1) & 1u, p.err)) break;
-            tc_fence_after();
-            const uint32_t trow = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * 256);
-            if (kF16 && !box && nst) {          // boxes become the staging buffer
+            uint32_t from = tmem_base;           // where the finished sums are
+            bool ok = true;
+            for (int s = 0; s < n_sums; s++) {
+                if (!mbar_wait_warp(&tfull[acc], acc_phase, p.err)) { ok = false; break; }
+                tc_fence_after();
+                if (n_sums == 1) {
+                    from = accumulator_at(acc);
+                } else {
+#pragma unroll 1
+                    for (int c = c0; c < c1; c++) {
+                        float v[32], w[32];
+                        const uint32_t sum = tmem_base + lanes + (uint32_t)(c * 32);
+                        tmem_ld32x2(accumulator_at(acc) + lanes + (uint32_t)(c * 32), v, sum, w);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] = s ? v[j] + w[j] : v[j];
+                        tmem_st32(sum, v);
+                    }
+                    release();
+                }
+            }
+            if (!ok) break;
+            if (kF16 && !box && nst) {           // boxes become the staging buffer
                 if (lane == 0) bulk_wait_group_read<0>();
                 __syncwarp();
             }
@@ -420,7 +501,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     const int cc = col0 + c * 32;
                     if (cc >= p.N) break;
                     float v[32];
-                    tmem_ld32(trow + (uint32_t)(c * 32), v);
+                    tmem_ld32(from + lanes + (uint32_t)(c * 32), v);
                     if (kF16 && box) {
                         store_box<EPI>(p, &tmC, v, bias, reinterpret_cast<uint8_t*>(stg) + (nst & 1u) * 2048, row0, cc);
                         nst++;
@@ -440,12 +521,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 }
                 __syncwarp();
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_remote(tempty_lead + (uint32_t)(ab * 8));
-                else mbar_arrive(&tempty[ab]);
-            }
+            if (n_sums == 1) release();
         }
         if (kF16) {      // the stores are complete before the CTA exits
             if (lane == 0) bulk_wait_group<0>();
