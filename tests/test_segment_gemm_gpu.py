@@ -185,10 +185,54 @@ def test_rows_of_no_utterance_get_the_projection_alone(K, synth, weights, lens, 
 
 
 @pytest.mark.parametrize("weights", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_F32_RESID])
+@pytest.mark.parametrize("N,Kd,lens", [(94, 576, [70, 1]), (320, 1088, [300, 40]), (1024, 2112, [499, 600, 801]), (200, 1024, [3, 64])])
+def test_long_sums(K, synth, weights, epi, N, Kd, lens):
+    """fp32 outputs over more of K than one tensor-core sum takes, whole and broken sums,
+    one and two accumulators beside the running total, adapters' blocks behind the last."""
+    c = Lora(K, synth, Segments(lens), [i % 2 for i in range(len(lens))], N, Kd, 24, 2, weights, epi)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_F32_RESID])
+@pytest.mark.parametrize("N,Kd", [(94, 576), (320, 2112), (200, 1024)])
+def test_grouped_long_sums(K, epi, N, Kd):
+    grouped(K, Segments([300, 1, 129, 64, 500]), [0, 2, 1, 1, 0], 3, N, Kd, epi)
+
+
+@pytest.mark.parametrize("weights", ["f16", "q8", "q4"])
 def test_many_adapters_in_one_tile(K, synth, weights):
     """Single frames of 300 streams with 40 adapters in no order: each row tile has nearly all of them."""
     rng = np.random.default_rng(3)
     c = Lora(K, synth, Segments([1] * 300), rng.integers(-1, 41, 300).tolist(), 256, 192, 16, 40, weights, EPI_F16)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("weights", ["f16", "q8"])
+@pytest.mark.parametrize("n_utt,top", [(129, 3), (1500, 3), (400, 40), (3000, 2), (700, 0)])
+def test_many_utterances(K, synth, weights, n_utt, top):
+    """More utterances than the planning threads, most of them short or empty, some long
+    ones among them, the first and last empty."""
+    rng = np.random.default_rng(n_utt)
+    lens = rng.integers(0, top + 1, n_utt)
+    lens[[n_utt // 3, n_utt // 2]] = [513, 130]
+    lens[0] = lens[-1] = 0
+    c = Lora(K, synth, Segments(lens.tolist(), gap=int(top == 2), tail=9), rng.integers(-1, 9, n_utt).tolist(), 136, 128, 16, 8, weights, EPI_F16)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("weights", ["f16", "q8"])
+def test_large_batch_uses_all_row_blocks(K, synth, weights):
+    """Enough rows for the 128-row blocks of the first product, utterance ends anywhere in them,
+    more than two adapters in some."""
+    rng = np.random.default_rng(4)
+    lens = rng.integers(1, 260, 160).tolist()
+    lens[40:60] = [7] * 20
+    c = Lora(K, synth, Segments(lens), rng.integers(-1, 12, 160).tolist(), 128, 192, 32, 12, weights, EPI_F32)
+    assert c.seg.M >= 128 * 148
     c.call()
     c.check()
 

@@ -28,7 +28,7 @@ static int pick_lora_tile(int N, int m_valid) {
 // Two epilogue warps per lane quarter for the heavier epilogues, as without adapters (launch_w).
 template <int EPI, int WQ>
 static int launch_lora(int bn, const QMaps& m, const QParams& p, const QLora<true>& lo, cudaStream_t st) {
-    constexpr int EH = EPI == W2V_EPI_F16_GELU || EPI == W2V_EPI_F32_RESID ? 2 : 1;
+    constexpr int EH = EPI == W2V_EPI_F16 ? 1 : 2;
     switch (bn) {
         case -192: return launch<192, EPI, WQ, true, EH, true>(m.x, m.q, m.s, m.c, m.r, p, st, lo);
         case -128: return launch<128, EPI, WQ, true, EH, true>(m.x, m.q, m.s, m.c, m.r, p, st, lo);
@@ -76,6 +76,9 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
     lo.t = lo.b = m.x;
     lo.lora = n_utt > 0;
     lo.plan = sg::lora_plan(workspace, M, n_utt, rank, rows, f16 ? 1 : 2);
+    // as the fp16 kernel does (segment_gemm.cu): 512 of K, 1024 beside a residual
+    lo.sum_blocks = epilogue == W2V_EPI_F32_RESID ? 16 : 8;
+    lo.n_sums = f16 ? 1 : (int)((K / kBK + lo.sum_blocks - 1) / lo.sum_blocks);
     lo.chunks = (2 * rank + code_row_bytes(wq) - 1) / code_row_bytes(wq);
     if (lo.lora) {
         if (lo.plan.parts * lo.plan.blocks * rows > 0x7fffffffLL) return W2V_ERR_ARGS;

@@ -81,6 +81,7 @@ struct QLora<true> {
     sg::LoraPlan plan;
     int chunks;          // k-blocks per adapter and part
     int lora;            // the plan holds adapters
+    int sum_blocks, n_sums;   // fp32 outputs: k-blocks of a sum, sums of a tile (segment_gemm.cu)
 };
 
 template <int BN, int WQ, bool PAIR, int EPI, int EH = 1>
@@ -205,6 +206,11 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
     const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
     const int n_units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int total = p.f_tiles * p.r_tiles;
+    // fp32 outputs beside adapters: accumulator 0 is then a running total that the epilogue
+    // warps add accumulator 1 to, every sum_blocks of K
+    constexpr bool SUMS = LORA && (EPI == W2V_EPI_F32 || EPI == W2V_EPI_F32_RESID);
+    [[maybe_unused]] bool sums = false;
+    if constexpr (SUMS) sums = lo.n_sums > 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) { mbar_init(&full[s], 1); mbar_init(&cfull[s], 1); mbar_init(&empty[s], 1); }
@@ -294,16 +300,32 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
             const uint32_t aempty_peer = PAIR ? mapa_shared(smem_u32(aempty), 1) : 0u;
             const uint32_t tfull_peer = PAIR ? mapa_shared(smem_u32(tfull), 1) : 0u;
             int stage = 0, it = 0, kq = 0;
+            [[maybe_unused]] int sum_it = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int tile = unit; tile < total && ok; tile += n_units, it++) {
-                const int ab = it & 1;
-                const uint32_t aph = (uint32_t)(it >> 1) & 1u;
+                int ab = it & 1;
+                uint32_t aph = (uint32_t)(it >> 1) & 1u;
+                if constexpr (SUMS) if (sums) { ab = 0; aph = (uint32_t)sum_it++ & 1u; }
                 if (!mbar_wait(&tempty[ab], aph ^ 1u, p.err)) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(ab * BN);
-                int n_kb = p.k_blocks;
+                uint32_t d = tmem_base + (uint32_t)(ab * BN);
+                if constexpr (SUMS) if (sums) d = tmem_base + (uint32_t)BN;
+                int n_kb = p.k_blocks, first_kb = 0;
                 for (int kb = 0; kb < n_kb; kb++, kq++) {
+                    if constexpr (SUMS)
+                        if (sums && kb && kb < p.k_blocks && kb % lo.sum_blocks == 0) {
+                            // hand the sum over and wait until it has been added
+                            if constexpr (PAIR) {
+                                umma_commit_pair(smem_u32(&tfull[0]));
+                                umma_commit_pair(tfull_peer);
+                            } else {
+                                umma_commit(&tfull[0]);
+                            }
+                            if (!mbar_wait(&tempty[0], ((uint32_t)sum_it++ & 1u) ^ 1u, p.err)) { ok = false; break; }
+                            tc_fence_after();
+                            first_kb = kb;
+                        }
                     const int f = kq % SB;
                     if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
                     const bool aok = PAIR ? mbar_wait_cluster(&afull[f], (uint32_t)(kq / SB) & 1u, p.err)
@@ -317,10 +339,10 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                         if (LORA && kb >= p.k_blocks && kk >= code_row_bytes(WQ) / 32) break;
                         if constexpr (PAIR)
                             umma_f16_pair_tmem_a(d, a0 + (uint32_t)(kk * 8), umma_desc_sw128(b0 + kk * 32), idesc,
-                                                 (kb | kk) != 0);
+                                                 kb != first_kb || kk != 0);
                         else
                             umma_f16_tmem_a(d, a0 + (uint32_t)(kk * 8), umma_desc_sw128(b0 + kk * 32), idesc,
-                                            (kb | kk) != 0);
+                                            kb != first_kb || kk != 0);
                     }
                     if constexpr (PAIR) {
                         umma_commit_pair(smem_u32(&empty[stage]));
@@ -440,6 +462,38 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
         // with EH = 2 two warps share a lane quarter and take alternate chunks (eh, eh + 2, ...)
         const int q = warp & 3;
         const int eh = (warp - 2) / 4;
+        [[maybe_unused]] int sum_it = 0;
+        // The tile's accumulator, complete; with sums in the running total, and handed back already.
+        auto take = [&](int ab, uint32_t aph, uint32_t tempty_lead, uint32_t& tacc) {
+            if constexpr (SUMS)
+                if (sums) {
+                    tacc = tmem_base + ((uint32_t)(32 * q) << 16);
+                    for (int s = 0; s < lo.n_sums; s++) {
+                        if (!mbar_wait(&tfull[0], (uint32_t)sum_it++ & 1u, p.err)) return false;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = eh; c < BN / 32; c += EH) {
+                            float v[32], w[32];
+                            tmem_ld32(tacc + (uint32_t)(BN + c * 32), v);
+                            tmem_ld32(tacc + (uint32_t)(c * 32), w);
+#pragma unroll
+                            for (int j = 0; j < 32; j++) v[j] = s ? v[j] + w[j] : v[j];
+                            tmem_st32(tacc + (uint32_t)(c * 32), v);
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (PAIR) mbar_arrive_remote(tempty_lead);
+                            else mbar_arrive(&tempty[0]);
+                        }
+                    }
+                    return true;
+                }
+            if (!mbar_wait(&tfull[ab], aph, p.err)) return false;
+            tc_fence_after();
+            tacc = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(ab * BN);
+            return true;
+        };
         if (p.tma) {
             // Staged: per 32 x 32 chunk, the residual box arrives by TMA R - 1 chunks
             // ahead (a ring of R boxes per warp, the first R - 1 requested before the
@@ -472,8 +526,9 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                 if (fcol0 >= p.N) {
                     // every feature of this warp's quarter is past the last one: nothing to
                     // load or store, only the accumulator to hand back
-                    if (!mbar_wait(&tfull[ab], aph, p.err)) break;
-                    tc_fence_after();
+                    uint32_t tacc;
+                    if (!take(ab, aph, tempty_lead, tacc)) break;
+                    if (sums) continue;
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
@@ -503,15 +558,14 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                 float2 stn = make_float2(0.f, 0.f);
                 if (EPI == W2V_EPI_F32_RESID_LN && ri * BN + eh * 32 + lane < p.m_valid)
                     stn = p.ln_stats[ri * BN + eh * 32 + lane];
-                if (!mbar_wait(&tfull[ab], aph, p.err)) break;
-                tc_fence_after();
-                const uint32_t tacc = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(ab * BN);
+                uint32_t tacc;
+                if (!take(ab, aph, tempty_lead, tacc)) break;
                 bool ok = true;
 #pragma unroll 1
                 for (int c = eh, k = 0; c < kNch; c += EH, k++) {
                     float v[32];
                     tmem_ld32(tacc + (uint32_t)(c * 32), v);
-                    if (c + EH >= kNch) {
+                    if (c + EH >= kNch && !sums) {
                         // this warp's last chunk is in registers: its share of the accumulator is free
                         tc_fence_before();
                         __syncwarp();
@@ -619,14 +673,13 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                 if (EPI == W2V_EPI_F32_RESID_LN) stn = r0 + lane < p.m_valid ? p.ln_stats[r0 + lane] : make_float2(0.f, 0.f);
             };
             if (kRes) fetch(eh);
-            if (!mbar_wait(&tfull[ab], aph, p.err)) break;
-            tc_fence_after();
-            const uint32_t tacc = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(ab * BN);
+            uint32_t tacc;
+            if (!take(ab, aph, tempty_lead, tacc)) break;
 #pragma unroll 1
             for (int c = eh; c < kNch; c += EH) {
                 float v[32];
                 tmem_ld32(tacc + (uint32_t)(c * 32), v);
-                if (c + EH >= kNch) {
+                if (c + EH >= kNch && !sums) {
                     // the accumulator is in registers: hand it back to the MMA
                     tc_fence_before();
                     __syncwarp();
