@@ -14,8 +14,8 @@
 // Arithmetic.  Probabilities are held as 64-bit numbers relative to the best
 // beam: each frame multiplies by exp(logit - row maximum) and rescales by a
 // power of two (exact), so that no logarithm or exponential stands in the
-// frame-to-frame chain.  The row maxima cancel, the powers of two and the
-// logarithms of the rows' sums are added up apart and enter the final score.
+// frame-to-frame chain.  The row maxima cancel; the powers of two are added up
+// apart and the rows' sums multiplied (and rescaled alike), for the final score.
 // Candidates below 2^-1000 of the frame's best are dropped, which also keeps
 // every held value a normal number.  Selecting on 64-bit values matters:
 // scores near the cut differ by less than 32 bits resolve after a few hundred
@@ -56,7 +56,8 @@ struct Header {
     int frames, nb;
     u64 tag;             // of a started state, with the sizes it was laid out for
     long long exp2;      // power of two taken out of the beams so far
-    double log_z;        // sum of the logarithms of the rows' sums
+    long long z_exp2;    // and out of z
+    double z;            // product of the rows' sums
 };
 
 // One beam, as the state keeps it between calls.
@@ -104,22 +105,26 @@ __host__ __device__ inline int pairs_of(int i, int V, int width) {
     return n < V - 1 ? n : V - 1;
 }
 
-// A frame's row as the search needs it: by_rank[n_tok], p[V], log_z.
+// A frame's row as the search needs it: by_rank[n_tok], key[V], p[V], z.
 struct Ranked {
     double p;            // exp(logit - max), largest first (equal ones by token)
     int tok, pad;
 };
 struct Row {
     Ranked* by_rank;
+    uint32_t* key;       // leading bits of p, 0 for blank and what cannot be emitted
     double* p;           // by token
-    double* log_z;       // logarithm of the sum of p (0: nothing can be emitted)
+    double* z;           // the sum of p (0: nothing can be emitted)
 };
-__host__ __device__ inline int row_bytes(int V, int width) { return (n_tokens(V, width) * 16 + (V + 1) * 8 + 15) / 16 * 16; }
+__host__ __device__ inline int row_bytes(int V, int width) {
+    return (n_tokens(V, width) * 16 + (V + 3) / 4 * 16 + (V + 1) * 8 + 15) / 16 * 16;
+}
 W2V_DEV Row row_at(uint8_t* base, int V, int n_tok) {
     Row r;
     r.by_rank = reinterpret_cast<Ranked*>(base);
-    r.p = reinterpret_cast<double*>(base + n_tok * 16);
-    r.log_z = r.p + V;
+    r.key = reinterpret_cast<uint32_t*>(base + n_tok * 16);
+    r.p = reinterpret_cast<double*>(base + n_tok * 16 + (V + 3) / 4 * 16);
+    r.z = r.p + V;
     return r;
 }
 
@@ -154,45 +159,19 @@ struct Shared {
     int slot[MW];                    // new place of an old beam that stays, -1: dropped
     int back[MW];                    // new beams whose node was found again
     int pair_at[MW];
-    uint16_t pair[max_live(MW) - MW];    // beam in the high byte, rank in the low
     int n_live, n_back, expired;
     int place_sum;                   // of the candidates: less than all different ones add up to where values are equal
     uint32_t least_hi[8];
     // of the last frame, for the hypotheses
     int nb, cur;
-    long long exp2;
-    double log_z;
+    long long exp2, z_exp2;
+    double z;
 };
 
 // A logit as the search sees it: NaN cannot be emitted, +inf is the largest number.
 W2V_DEV float clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
 W2V_DEV u64 bits_of(double x) { return (u64)__double_as_longlong(x); }   // positive numbers order as their bits
 W2V_DEV double value_of(u64 k) { return __longlong_as_double((long long)k); }
-
-// Row producer: one warp turns the logits of a frame into a Row.
-W2V_DEV void make_row(const float* x, int V, int blank, int n_tok, float mx, const Row& r) {
-    const int lane = threadIdx.x & 31;
-    double z = 0.0;
-    for (int v = lane; v < V; v += 32) {
-        const float l = clean(x[v]);
-        const double e = l == -INFINITY ? 0.0 : exp((double)l - (double)mx);
-        r.p[v] = e;
-        z += e;
-    }
-    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    __syncwarp();
-    for (int v = lane; v < V; v += 32) {
-        const u64 e = bits_of(r.p[v]);
-        int rank = 0;
-        for (int w = 0; w < V; w++) {
-            const u64 f = bits_of(r.p[w]);
-            rank += w != blank && (w < v ? f >= e : f > e);
-        }
-        if (v != blank && rank < n_tok) r.by_rank[rank] = Ranked{value_of(e), v, 0};
-    }
-    if (lane == 0) *r.log_z = z > 0.0 ? log(z) : 0.0;
-    __syncwarp();
-}
 
 // The best candidate of a frame is at least half and less than four times the
 // best beam, which is held between 1 and 2: what is to be kept lies between
@@ -201,12 +180,76 @@ W2V_DEV void make_row(const float* x, int V, int blank, int n_tok, float mx, con
 constexpr u64 kLeast = (u64)20 << 52;
 W2V_DEV uint32_t leading(u64 k) { return (uint32_t)((k - kLeast) >> 30); }
 
+// Row producer: one warp turns the logits of a frame into a Row.  Tokens are
+// ranked by how many have larger leading bits, four keys a load; where two have
+// the same (one frame in a thousand), by the whole values and the id.
+W2V_DEV void make_row(const float* x, int V, int blank, int n_tok, float mx, const Row& r) {
+    const int lane = threadIdx.x & 31, V4 = (V + 3) / 4;
+    double z = 0.0;
+    for (int v = lane; v < 4 * V4; v += 32) {
+        const float l = v < V ? clean(x[v]) : -INFINITY;
+        const double e = l == -INFINITY ? 0.0 : exp((double)l - (double)mx);
+        if (v < V) r.p[v] = e;
+        r.key[v] = v != blank && bits_of(e) >= kLeast ? leading(bits_of(e)) : 0;
+        z += e;
+    }
+    for (int v = lane; v < n_tok; v += 32) r.by_rank[v] = Ranked{0.0, blank ? 0 : 1, 0};    // (fewer can be emitted)
+    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    __syncwarp();
+    int ranks = 0, some = 0;
+    for (int v = lane; v < V; v += 32) {
+        const uint32_t k = r.key[v];
+        int c0 = 0, c1 = 0;
+#pragma unroll 8
+        for (int w = 0; w < V4; w++) {
+            const uint4 q = reinterpret_cast<const uint4*>(r.key)[w];
+            c0 += (q.x > k) + (q.y > k);
+            c1 += (q.z > k) + (q.w > k);
+        }
+        if (k) {
+            ranks += c0 + c1;
+            some++;
+            if (c0 + c1 < n_tok) r.by_rank[c0 + c1] = Ranked{r.p[v], v, 0};
+        }
+    }
+    ranks = __reduce_add_sync(0xffffffffu, ranks);
+    some = __reduce_add_sync(0xffffffffu, some);
+    if (ranks != some * (some - 1) / 2)
+        for (int v = lane; v < V; v += 32) {
+            const u64 e = bits_of(r.p[v]);
+            int rank = 0;
+            for (int w = 0; w < V; w++) {
+                const u64 f = bits_of(r.p[w]);
+                rank += w != blank && (w < v ? f >= e : f > e);
+            }
+            if (v != blank && rank < n_tok) r.by_rank[rank] = Ranked{value_of(e), v, 0};
+        }
+    if (lane == 0) *r.z = z;
+    __syncwarp();
+}
+
+// 2^-1000 of the best.
+W2V_DEV u64 pruned(u64 best) { return best > ((u64)1000 << 52) ? best - ((u64)1000 << 52) : 0; }
+constexpr int kExtends = 1 << 16;    // in n_live, above the number: extensions among them (whatever multiple)
+
 // Barrier of the NC search warps.
 template <int NC>
 W2V_DEV void search_sync() {
     if (NC == 1) __syncwarp();
     else asm volatile("barrier.sync 1, %0;" ::"n"(NC * 32) : "memory");
 }
+// Whether x holds for any thread of the search warps (a barrier too).
+template <int NC>
+W2V_DEV bool search_any(bool x) {
+    int r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.red.or.pred q, 1, %2, p;\n selp.s32 %0, 1, 0, q;\n}"
+        : "=r"(r)
+        : "r"((int)x), "n"(NC * 32)
+        : "memory");
+    return r != 0;
+}
+
 // How many of the keys are larger than k: 32 of every `step`, as long as they
 // begin before n (keys behind the last are 0).
 W2V_DEV int count_above(const uint32_t* keys, int n, int step, uint32_t k) {
@@ -225,9 +268,10 @@ W2V_DEV int count_above(const uint32_t* keys, int n, int step, uint32_t k) {
 }
 
 // NC search warps (the chain from frame to frame; beam i is thread i's) and
-// NP row producers (frame t: warp t % NP), a ring of rows between them.
+// NP row producers (frame t: warp t % NP), a ring of rows between them; one more
+// warp multiplies the rows' sums, which nothing in the chain needs.
 template <int NC, int NP, int MW>
-__global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
+__global__ void __launch_bounds__((NC + NP + 1) * 32, 1) ctc_beam_kernel(Params p) {
     constexpr int NT = NC * 32;
     constexpr int kPairs = (max_live(MW) - MW + NT - 1) / NT;       // of a thread
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -247,69 +291,64 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
     const int T = p.T[u] > 0 ? p.T[u] : 0;
     int frames = 0, nb = 1;
     long long exp2 = 0;
-    double log_z = 0.0;
     const u64 tag = tag_of(V, p.blank, W, p.max_frames);
     bool refused = p.resume && hdr->tag != tag;      // not a state of such a search
     if (p.resume && !refused) {
         frames = hdr->frames;
         nb = hdr->nb;
         exp2 = hdr->exp2;
-        log_z = hdr->log_z;
     }
     refused = refused || T > p.max_frames - frames;
     if (refused && tid == 0) report_error(p.err, kErrBadArgs);
-    for (int i = tid; i < W * words; i += (NC + NP) * 32) bits[i] = 0;
-    for (int i = tid; i < max_live(MW); i += (NC + NP) * 32) s.key32[i] = 0;
     if (tid < 2 * NP) {
         mbar_init(&full[tid], 1);
-        mbar_init(&empty[tid], 1);
+        mbar_init(&empty[tid], 2);       // search warps and the product of sums
+        fence_mbar_init();
     }
     if (tid == 0) {
-        fence_mbar_init();
         s.n_live = 0;
         s.n_back = 0;
         s.expired = 0;
         s.place_sum = 0;
     }
-    if (warp == 0) {         // where each beam's pairs start
-        int before = 0;
-        for (int i0 = 0; i0 < W; i0 += 32) {
-            const int n = i0 + lane < W ? pairs_of(i0 + lane, V, W) : 0;
-            int incl = n;
-            for (int d = 1; d < 32; d <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= d) incl += v;
-            }
-            if (i0 + lane < W) s.pair_at[i0 + lane] = before + incl - n;
-            before += __shfl_sync(0xffffffffu, incl, 31);
-        }
-    }
-    __syncthreads();
-    for (int i = warp; i < W; i += NC + NP)
-        for (int k = lane; k < pairs_of(i, V, W); k += 32) s.pair[s.pair_at[i] + k] = (uint16_t)(i << 8 | k);
-    double my_pb = 0.0, my_pn = 0.0, my_total = 0.0;     // this thread's beam
-    int my_last = -1, my_par = -1;
-    if (tid < nb && !refused) {
-        SavedBeam v{1.0, 0.0, 0, 0, -1, 0, -1, -1, -1};
-        if (p.resume) v = saved[tid];
-        else nodes[0] = Node{-1, -1, -1, -1};
-        my_pb = v.pb;
-        my_pn = v.pn;
-        my_total = my_pb + my_pn;
-        my_last = v.last;
-        my_par = v.par;
-        s.beams[0].prob[tid] = {my_pb, my_total};
-        s.beams[0].pn[tid] = my_pn;
-        s.beams[0].info[tid] = {v.node, v.last, v.len, v.pnode};
-        s.beams[0].link[tid] = {{(uint32_t)v.mask, (uint32_t)(v.mask >> 32)}, v.head, v.par};
-        if (my_par >= 0) atomicOr(&bits[my_par * words + (my_last >> 5)], 1u << (my_last & 31));
-    }
-    __syncthreads();
+    __syncthreads();                     // the row producers need no more
 
     const int n_frames = refused ? 0 : T;
     const float* x = p.logits + p.off[u] * V;
     const int rbytes = row_bytes(V, W);
-    if (warp >= NC) {
+    if (warp == NC + NP) {
+        double z = 1.0;
+        long long z_exp2 = 0;
+        bool ok = true;
+        if (p.resume && !refused) {
+            z = hdr->z;
+            z_exp2 = hdr->z_exp2;
+        }
+        int sl = 0;
+        uint32_t odd = 0;
+        for (int t = 0; t < n_frames && ok; t++) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[sl], odd, p.err));
+            if (!ok) break;
+            const double row_z = *row_at(rows + sl * rbytes, V, n_tok).z;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[sl]);
+            if (row_z > 0.0) {               // (0: no hypothesis is left)
+                const u64 v = bits_of(z * row_z);
+                const int e = (int)(v >> 52) - 1023;
+                z = value_of(v - ((u64)e << 52));
+                z_exp2 += e;
+            }
+            if (++sl == p.slots) { sl = 0; odd ^= 1u; }
+        }
+        if (lane == 0) {
+            s.z = z;
+            s.z_exp2 = z_exp2;
+            if (!refused && ok) {
+                hdr->z = z;
+                hdr->z_exp2 = z_exp2;
+            }
+        }
+    } else if (warp >= NC) {
         int sl = warp - NC;              // slot of the frame, and whether the ring's rounds so far are odd
         uint32_t odd = 0;
         for (int t = warp - NC; t < n_frames; t += NP) {
@@ -324,13 +363,51 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
             if (sl >= p.slots) { sl -= p.slots; odd ^= 1u; }
         }
     } else {
+        for (int i = tid; i < W * words; i += NT) bits[i] = 0;
+        for (int i = tid; i < max_live(MW); i += NT) s.key32[i] = 0;
+        if (warp == 0) {                 // where each beam's pairs start
+            int before = 0;
+            for (int i0 = 0; i0 < MW; i0 += 32) {
+                const int n = i0 + lane < W ? pairs_of(i0 + lane, V, W) : 0;
+                int incl = n;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+                    if (lane >= d) incl += v;
+                }
+                s.pair_at[i0 + lane] = before + incl - n;
+                before += __shfl_sync(0xffffffffu, incl, 31);
+            }
+        }
+        double my_pb = 0.0, my_pn = 0.0, my_total = 0.0;     // this thread's beam
+        int my_last = -1, my_par = -1;
+        search_sync<NC>();
+        if (tid < nb && !refused) {
+            SavedBeam v{1.0, 0.0, 0, 0, -1, 0, -1, -1, -1};
+            if (p.resume) v = saved[tid];
+            else nodes[0] = Node{-1, -1, -1, -1};
+            my_pb = v.pb;
+            my_pn = v.pn;
+            my_total = my_pb + my_pn;
+            my_last = v.last;
+            my_par = v.par;
+            s.beams[0].prob[tid] = {my_pb, my_total};
+            s.beams[0].pn[tid] = my_pn;
+            s.beams[0].info[tid] = {v.node, v.last, v.len, v.pnode};
+            s.beams[0].link[tid] = {{(uint32_t)v.mask, (uint32_t)(v.mask >> 32)}, v.head, v.par};
+            if (my_par >= 0) atomicOr(&bits[my_par * words + (my_last >> 5)], 1u << (my_last & 31));
+        }
         int pi[kPairs], pj[kPairs];      // this thread's extensions (beam, rank), beam MW: none
 #pragma unroll
         for (int e = 0; e < kPairs; e++) {
             const int c = e * NT + tid;
-            pi[e] = c < p.n_pairs ? s.pair[c] >> 8 : MW;
-            pj[e] = c < p.n_pairs ? s.pair[c] & 255 : 0;
+            int i = 0;                   // the last beam whose pairs start at or before c
+#pragma unroll
+            for (int d = MW / 2; d; d /= 2)
+                if (i + d < W && s.pair_at[i + d] <= c) i += d;
+            pi[e] = c < p.n_pairs ? i : MW;
+            pj[e] = c < p.n_pairs ? c - s.pair_at[i] : 0;
         }
+        search_sync<NC>();
         int sl = 0, cur = 0;
         uint32_t odd = 0;
         bool ready = false;              // the frame's row was seen to be complete
@@ -362,17 +439,19 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
             // the stays, and each beam's best candidate: `width` different ones, so the
             // least of them bounds from below what can be kept
             u64 stay = 0, most = ~(u64)0;
+            double stay_b = 0.0, stay_n = 0.0;
             if (tid < nb) {
                 const double from = my_par >= 0 ? my_pn + (above_last == my_last ? above.pb : above.total) : my_pn;
-                const double sb = my_total * p_blank, sn = my_last >= 0 ? from * p_last : 0.0;
-                stay = bits_of(sb + sn);
+                stay_b = my_total * p_blank;
+                stay_n = my_last >= 0 ? from * p_last : 0.0;
+                stay = bits_of(stay_b + stay_n);
                 most = stay;
                 // no more than two looked at: the likeliest token is as a rule neither a beam's already nor the beam's last
                 const u64 e0 = bits_of((k0.tok == my_last ? my_pb : my_total) * k0.p);
                 const u64 e1 = bits_of((k1.tok == my_last ? my_pb : my_total) * k1.p);
                 if (!(w0 & 1u) && e0 > most) most = e0;
                 if (!(w1 & 1u) && e1 > most) most = e1;
-                s.stay[tid] = {sb, sn};
+                s.stay[tid] = {stay_b, stay_n};
                 s.slot[tid] = -1;
             }
             uint32_t least = __reduce_min_sync(0xffffffffu, (uint32_t)(most >> 32));
@@ -402,10 +481,41 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
                 in[e] = __ballot_sync(0xffffffffu, k >= kLeast && (uint32_t)(k >> 32) >= least);
                 total_in += __popc(in[e]);
             }
+            // Only stays, in the order they had (most blank frames): the beams keep their places,
+            // tokens and nodes, and no more than their probabilities change.
+            uint32_t extends = 0;
+#pragma unroll
+            for (int e = 0; e < kPairs; e++) extends |= in[e];
+            auto unchanged = [&](u64 best, u64 next) {
+                return tid >= nb || (stay >= kLeast && stay >= pruned(best) && (tid + 1 == nb || stay >= next));
+            };
+            auto keep_places = [&](u64 best) {
+                const int e2 = (int)(best >> 52) - 1023;
+                const double scale = value_of((u64)(1023 - e2) << 52);
+                if (tid < nb) {
+                    my_pb = stay_b * scale;
+                    my_pn = stay_n * scale;
+                    my_total = my_pb + my_pn;
+                    s.beams[cur].prob[tid] = {my_pb, my_total};
+                    s.beams[cur].pn[tid] = my_pn;
+                }
+                if (tid == 0) mbar_arrive(&empty[sl]);
+                exp2 += e2;
+                if (++sl == p.slots) { sl = 0; odd ^= 1u; }
+                ready = t + 1 < n_frames && mbar_try_wait(&full[sl], odd);
+            };
+            if (NC == 1 && nb && !extends) {
+                const u64 best = __shfl_sync(0xffffffffu, stay, 0), next = __shfl_down_sync(0xffffffffu, stay, 1);
+                if (__all_sync(0xffffffffu, unchanged(best, next))) {
+                    keep_places(best);
+                    __syncwarp();
+                    continue;
+                }
+            }
             if (NC == 1 || total_in) {
                 int at = 0;
                 if (NC > 1) {
-                    if (lane == 0) at = atomicAdd(&s.n_live, total_in);
+                    if (lane == 0) at = atomicAdd(&s.n_live, total_in | (extends ? kExtends : 0)) & (kExtends - 1);
                     at = __shfl_sync(0xffffffffu, at, 0);
                 }
 #pragma unroll
@@ -421,7 +531,18 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
                 }
             }
             search_sync<NC>();
-            const int live = NC == 1 ? total_in : s.n_live;
+            const int live = NC == 1 ? total_in : s.n_live & (kExtends - 1);
+            if (NC > 1 && nb && live == s.n_live) {
+                const u64 best = bits_of(s.stay[0].b + s.stay[0].n);
+                const u64 next = tid + 1 < nb ? bits_of(s.stay[tid + 1].b + s.stay[tid + 1].n) : 0;
+                if (!search_any<NC>(!unchanged(best, next))) {
+                    for (int a = tid; a < live; a += NT) s.key32[a] = 0;
+                    if (tid == 0) s.n_live = 0;
+                    keep_places(best);
+                    search_sync<NC>();
+                    continue;
+                }
+            }
             // their places in order: how many have larger leading bits (which decide but for one
             // frame in some hundreds)
             auto put = [&](int c, int a) {
@@ -493,7 +614,7 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
             const u64 best = nn ? s.sel[0].key : 0;
             const int e2 = nn ? (int)(best >> 52) - 1023 : 0;
             const double scale = value_of((u64)(1023 - e2) << 52);
-            const u64 floor = best > ((u64)1000 << 52) ? best - ((u64)1000 << 52) : 0;
+            const u64 floor = pruned(best);
             while (nn && s.sel[nn - 1].key < floor) nn--;
             const int my_slot = tid < nb ? s.slot[tid] : 0;
             const bool drops = tid < nb && (uint32_t)my_slot >= (uint32_t)nn;
@@ -542,7 +663,6 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
                 n.link[tid] = {{mask0, mask1}, head, par};
             }
             for (int a = tid; a < live; a += NT) s.key32[a] = 0;
-            if (tid == 0) log_z += *r.log_z;
             search_sync<NC>();
             if (tid == 0) {
                 mbar_arrive(&empty[sl]);
@@ -581,7 +701,6 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
             s.nb = refused || failed ? 0 : nb;
             s.cur = cur;
             s.exp2 = exp2;
-            s.log_z = log_z;
             if (failed) hdr->tag = 0;
         }
         // state for the next call
@@ -591,7 +710,6 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
                 hdr->nb = nb;
                 hdr->tag = tag;
                 hdr->exp2 = exp2;
-                hdr->log_z = log_z;
             }
             if (tid < nb) {
                 const auto info = s.beams[cur].info[tid];
@@ -605,14 +723,15 @@ __global__ void __launch_bounds__((NC + NP) * 32, 1) ctc_beam_kernel(Params p) {
     // hypotheses, best first
     const Beams<MW>& b = s.beams[s.cur];
     const int have = s.nb < p.n_best ? s.nb : p.n_best;
-    for (int h = warp; h < p.n_best; h += NC + NP) {
+    for (int h = warp; h < p.n_best; h += NC + NP + 1) {
         const long long at = (long long)u * p.n_best + h;
         const int len = h < have ? b.info[h].len : -1;
         int* out = p.ids + at * p.cap;
         for (long long i = (len > 0 ? len : 0) + lane; i < p.cap; i += 32) out[i] = -1;
         if (lane) continue;
         p.n_ids[at] = len;
-        p.scores[at] = h < have ? log(b.prob[h].total) + (double)s.exp2 * 0.69314718055994530942 - s.log_z : -INFINITY;
+        p.scores[at] = h < have ? log(b.prob[h].total) - log(s.z) + (double)(s.exp2 - s.z_exp2) * 0.69314718055994530942
+                               : -INFINITY;
         if (len > 0)
             for (int i = len - 1, id = b.info[h].node; i >= 0; i--) {
                 const Node nd = nodes[id];
@@ -637,7 +756,7 @@ static int launch(Params p, int n_utt, cudaStream_t st) {
             return W2V_ERR_LAUNCH;
         attr[dev & 63] = true;
     }
-    kern<<<n_utt, (NC + NP) * 32, smem, st>>>(p);
+    kern<<<n_utt, (NC + NP + 1) * 32, smem, st>>>(p);
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
 
@@ -681,6 +800,8 @@ extern "C" int w2v_ctc_beam(const float* logits, const long long* off, const int
     p.n_pairs = 0;
     for (int i = 0; i < width; i++) p.n_pairs += pairs_of(i, V, width);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    // up to 32 beams one warp searches, without barriers
-    return width <= 32 ? launch<1, 4, 32>(p, n_utt, st) : launch<8, 8, 128>(p, n_utt, st);
+    // Up to 32 beams one warp searches, without barriers, and takes about a microsecond a frame;
+    // a row of 32 tokens costs a producer half of that, one of 200 ten times as much.
+    if (width <= 32) return V <= 64 ? launch<1, 2, 32>(p, n_utt, st) : launch<1, 7, 32>(p, n_utt, st);
+    return launch<8, 7, 128>(p, n_utt, st);
 }
