@@ -128,7 +128,8 @@ def ctc_logits(rng, T, V, blank, peak=6.0):
 @pytest.mark.parametrize("V,width,n_best,lens,blank", [
     (32, 16, 4, [60, 0, 1, 33], 0), (32, 1, 1, [80, 5], 0), (2, 5, 5, [40, 1], 0), (3, 8, 8, [50], 1), (32, 2, 2, [70], 31),
     (5, 128, 10, [40, 12], 2), (32, 100, 10, [50, 3], 0), (64, 33, 3, [40], 7), (94, 20, 2, [45, 2], 0), (200, 9, 9, [30], 199),
-    (1024, 4, 2, [12], 3), (33, 127, 127, [20], 0), (31, 31, 31, [25], 30)])
+    (1024, 4, 2, [12], 3), (33, 127, 127, [20], 0), (31, 31, 31, [25], 30), (300, 100, 5, [12], 0),
+    (65, 32, 3, [30, 9], 64), (70, 34, 3, [25], 1), (258, 128, 4, [9], 7)])
 def test_hypotheses_and_scores(K, V, width, n_best, lens, blank):
     rng = np.random.default_rng(V * 1000 + width)
     logits = [ctc_logits(rng, t, V, blank) for t in lens]
