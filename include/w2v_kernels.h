@@ -220,6 +220,8 @@ int w2v_ctc_greedy(const float* logits, const long long* off, const int* T, int 
  *   workspace: device memory of w2v_lora_workspace_bytes(M, n_utt, rank)
  *      bytes, 128-byte aligned, not shared by calls that may overlap.
  *      W2V_ERR_CAPACITY when it is too small.
+ * lora_b of an adapter in use must be finite: an infinity or NaN there may
+ * reach the rows of other utterances nearby (at most 256 rows away).
  * A, W, lora_a, lora_b (and Bs) 16-byte aligned.  s_a lora_a[a] A[r] is held
  * in fp16 (as two numbers, value and remainder, for the fp32 epilogues): its
  * magnitude must stay below 65504. */

@@ -71,6 +71,17 @@ int wav2vec2_b200_forward_device(struct wav2vec2_context * ctx, const float * d_
 int wav2vec2_b200_device_outputs(struct wav2vec2_context * ctx, const float ** logits,
                                  const int ** spans, const int ** n_spans, long long * M);
 
+/* Prefix beam search over the logits of the last forward_device batch, on the
+ * device (w2v_ctc_beam; wav2vec2_b200_ctc_beam_search is the host's): the
+ * n_best most likely hypotheses of every utterance, 1 <= n_best <= beam_width
+ * <= 128.  All outputs are device memory: n_ids and scores [n_utt][n_best]
+ * (tokens of a hypothesis, -1 where there are fewer; its natural-log
+ * probability), ids [n_utt][n_best][cap] (the first cap tokens, -1 behind
+ * them).  Enqueues on `stream`, which must follow the forward's (NULL: the
+ * context's own stream, as there), and returns without synchronising. */
+int wav2vec2_b200_beam_device(struct wav2vec2_context * ctx, int beam_width, int n_best, int * ids, long long cap,
+                              int * n_ids, double * scores, void * stream);
+
 /* Stage-wise activations of one utterance for parity checks (fp32, host):
  * feat [T, conv_dim] (extractor output), stages [(n_layers + 2), T, hidden]:
  * block 0 = feature projection, 1 = after positional conv (+ encoder LN for

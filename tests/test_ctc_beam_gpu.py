@@ -329,3 +329,78 @@ def test_captured_and_on_two_streams(K):
     g.replay()
     g.replay()
     b.check([x[::-1] for x in sets[0]])
+
+
+def test_beam_of_a_forward(K, pkg, model_path, synth):
+    """wav2vec2_b200_beam_device: the hypotheses of the last forward's logits, on the
+    forward's stream; an utterance too short for a frame has the empty one."""
+    import w2v_b200.binding as B
+    m = B.Model(model_path("tiny", "q8_0", bias_std=0.02, gain_jitter=0.1))
+    xs = [synth.make_audio(n, 40 + i) for i, n in enumerate([9000, 300, 14000, 4321])]
+    d = torch.from_numpy(np.concatenate(xs)).cuda()
+    n, best, width, cap = len(xs), 3, 6, 60
+    ids = torch.full((n, best, cap), -7, dtype=torch.int32, device="cuda")
+    n_ids = torch.full((n, best), -7, dtype=torch.int32, device="cuda")
+    scores = torch.zeros(n, best, dtype=torch.float64, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):                                # (the later forwards are replayed graphs)
+        m.forward_device(d.data_ptr(), [len(x) for x in xs], s.cuda_stream)
+        m.beam_device(width, best, ids.data_ptr(), cap, n_ids.data_ptr(), scores.data_ptr(), s.cuda_stream)
+    torch.cuda.synchronize()
+    assert m.n_frames(300) == 0
+    for u, lg in enumerate(m.logits(xs)):
+        ref = search(lg, m.cfg["pad_id"], width)[:best]
+        got = [(tuple(ids[u, h, :int(n_ids[u, h])].tolist()), float(scores[u, h])) for h in range(best) if n_ids[u, h] >= 0]
+        assert [g[0] for g in got] == [r[0] for r in ref], u
+        assert all(abs(g[1] - r[1]) <= 1e-9 * (1 + abs(r[1])) for g, r in zip(got, ref))
+    for bad in ((0, 1), (129, 1), (4, 5), (4, 0)):
+        with pytest.raises(B.EngineError):
+            m.beam_device(*bad, ids.data_ptr(), cap, n_ids.data_ptr(), scores.data_ptr())
+    with pytest.raises(B.EngineError):
+        m.beam_device(4, 1, 0, cap, n_ids.data_ptr(), scores.data_ptr())
+    m.close()
+
+
+def test_adapters_heads_and_beams_together(K):
+    """One batch of utterances in three languages: a shared projection with an adapter for
+    each, an output head for each, and the beams over the logits; logits and hypotheses
+    against the same in 64 bits (the search on the logits that came out)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    lens, lang = [37, 0, 64, 21, 50], [2, 0, 1, 0, 2]
+    M, Kd, H, V, rank = sum(lens), 192, 256, 24, 16
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    x, w, bias = r(M, Kd).half(), (r(H, Kd) / Kd ** 0.5).half(), r(H)
+    la, lb = (r(3, rank, Kd) / Kd ** 0.5).half(), (r(3, H, rank) / rank ** 0.5).half()
+    head, hb = (r(3, V, H) * 3 / H ** 0.5).half(), r(3, V)
+    off = torch.tensor(np.concatenate([[0], np.cumsum(lens)[:-1]]), dtype=torch.int64, device="cuda")
+    T, which = torch.tensor(lens, dtype=torch.int32, device="cuda"), torch.tensor(lang, dtype=torch.int32, device="cuda")
+    h = torch.empty(M, H, dtype=torch.float16, device="cuda")
+    logits = torch.empty(M, V, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    work = torch.empty(K.lora_workspace_bytes(M, 5, rank), dtype=torch.uint8, device="cuda")
+    state = torch.empty(K.ctc_beam_state_bytes(5, V, 8, 64), dtype=torch.uint8, device="cuda")
+    ids = torch.empty(5, 2, 64, dtype=torch.int32, device="cuda")
+    n_ids, scores = torch.empty(5, 2, dtype=torch.int32, device="cuda"), torch.empty(5, 2, dtype=torch.float64, device="cuda")
+    K.gemm_lora(x.data_ptr(), Kd, Kd, M, w.data_ptr(), H, h.data_ptr(), H, bias.data_ptr(), 0, H, 1, la.data_ptr(), lb.data_ptr(), 0,
+                3, rank, off.data_ptr(), T.data_ptr(), which.data_ptr(), 5, work.data_ptr(), work.numel(), err.data_ptr(), st())
+    K.gemm_grouped(h.data_ptr(), H, H, M, head.data_ptr(), 3, V, logits.data_ptr(), V, hb.data_ptr(), 0, V, 2, off.data_ptr(),
+                   T.data_ptr(), which.data_ptr(), 5, err.data_ptr(), st())
+    K.ctc_beam(logits.data_ptr(), off.data_ptr(), T.data_ptr(), 5, V, 0, 8, 64, False, state.data_ptr(), state.numel(), 2,
+               ids.data_ptr(), 64, n_ids.data_ptr(), scores.data_ptr(), err.data_ptr(), st())
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    at = 0
+    for u, (t, e) in enumerate(zip(lens, lang)):
+        xs = x[at:at + t].double()
+        z = xs @ w.double().T + bias.double() + (xs @ la[e].double().T) @ lb[e].double().T
+        z = 0.5 * z * (1 + torch.tanh(0.7978845608028654 * (z + 0.044715 * z ** 3)))
+        ref = z @ head[e].double().T + hb[e].double()
+        # h is rounded to fp16 (2^-11) and its products, at most |h| |head|, are summed
+        near = 2.0 ** -10 * (z.abs() @ head[e].double().abs().T) + 1e-3
+        got = logits[at:at + t].double()
+        assert ((got - ref).abs() <= near).all()
+        hyps = search(logits[at:at + t].cpu().numpy(), 0, 8)[:2]
+        assert [tuple(ids[u, i, :int(n_ids[u, i])].tolist()) for i in range(len(hyps))] == [q[0] for q in hyps]
+        assert all(abs(float(scores[u, i]) - q[1]) <= 1e-9 * (1 + abs(q[1])) for i, q in enumerate(hyps))
+        at += t

@@ -50,6 +50,7 @@ SIGNATURES = {
     "wav2vec2_b200_logits": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
     "wav2vec2_b200_forward_device": (_i, [_vp, _vp, _vp, _i, _vp]),
     "wav2vec2_b200_device_outputs": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "wav2vec2_b200_beam_device": (_i, [_vp, _i, _i, _vp, _ll, _vp, _vp, _vp]),
     "wav2vec2_b200_debug_stages": (_i, [_vp, _vp, _i, _vp, _vp, _vp]),
     "wav2vec2_b200_profile": (_i, [_vp, _i]),
     "wav2vec2_b200_profile_read": (_i, [_vp, _vp, _vp, _vp, _vp, _i]),
@@ -246,6 +247,14 @@ class Model:
     def forward_device(self, d_audio: int, n_samples, stream: int = 0) -> None:
         n = (C.c_int * len(n_samples))(*[int(x) for x in n_samples])
         rc = lib().wav2vec2_b200_forward_device(self.h, d_audio, C.cast(n, _vp), len(n_samples), stream or None)
+        if rc:
+            raise EngineError(last_error())
+
+    def beam_device(self, beam_width: int, n_best: int, ids: int, cap: int, n_ids: int, scores: int,
+                    stream: int = 0) -> None:
+        """Hypotheses of the last forward_device batch (device pointers; wav2vec2_b200_beam_device)."""
+        rc = lib().wav2vec2_b200_beam_device(self.h, beam_width, n_best, ids or None, cap, n_ids or None,
+                                             scores or None, stream or None)
         if rc:
             raise EngineError(last_error())
 

@@ -507,6 +507,24 @@ int wav2vec2_b200_profile_read(wav2vec2_context* ctx, const char** names, double
     return ctx->engines[0]->profile_read(names, ms, launches, flops, cap);
 }
 
+int wav2vec2_b200_beam_device(wav2vec2_context* ctx, int beam_width, int n_best, int* ids, long long cap, int* n_ids,
+                              double* scores, void* stream) {
+    if (!ctx) {
+        set_error("invalid arguments");
+        return W2V_STATUS_INVALID;
+    }
+    try {
+        if (!ctx->engines[0]->beam(beam_width, n_best, ids, cap, n_ids, scores, reinterpret_cast<cudaStream_t>(stream))) {
+            set_error("invalid arguments");
+            return W2V_STATUS_INVALID;
+        }
+    } catch (const std::exception& ex) {
+        set_error(ex.what());
+        return W2V_STATUS_CUDA;
+    }
+    return W2V_STATUS_OK;
+}
+
 int wav2vec2_b200_ctc_beam_search(const float* logits, int T, int V, int blank, int beam_width, int* ids,
                                   int cap) {
     if (T < 0 || V <= 0 || blank < 0 || blank >= V || beam_width < 1 || cap < 0 || (T > 0 && !logits) ||

@@ -509,6 +509,21 @@ void Engine::upload_meta(const BatchGeom& g, cudaStream_t st) {
     cuda_check(cudaEventRecord(meta_done_, st), "meta event");
 }
 
+bool Engine::beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st) {
+    cuda_check(cudaSetDevice(device_), "cudaSetDevice");
+    if (!st) st = stream_;
+    const int frames = std::max(last_T_max_, 1);
+    const long long bytes = w2v_ctc_beam_state_bytes(last_n_utt_, cfg_.vocab, width, frames);
+    if (bytes < 0 || n_best < 1 || n_best > width || !ids || !n_ids || !scores || cap < 1) return false;
+    if (last_n_utt_ == 0) return true;
+    beam_state_.ensure((size_t)bytes);
+    const int rc = w2v_ctc_beam(logits_.as<float>(), d_T_off_, d_T_, last_n_utt_, cfg_.vocab, cfg_.pad_id, width, frames, 0,
+                                beam_state_.p, bytes, n_best, ids, cap, n_ids, scores, err_.as<int>(), st);
+    if (rc == W2V_ERR_ARGS) return false;
+    if (rc != W2V_OK) throw std::runtime_error("ctc_beam: status " + std::to_string(rc));
+    return true;
+}
+
 int Engine::check_device_error() {
     int e = 0;
     cudaSetDevice(device_);
@@ -527,6 +542,8 @@ int Engine::check_device_error() {
 bool Engine::fwd_begin(const BatchGeom& g, cudaStream_t st) {
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     last_M_ = g.M;
+    last_n_utt_ = g.n_utt;
+    last_T_max_ = g.T_max;
     launches_cur_ = 0;
     if (g.n_utt == 0) { launches_last_ = 0; return false; }
     ensure_workspace(g);

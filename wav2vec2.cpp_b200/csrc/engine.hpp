@@ -108,6 +108,10 @@ public:
     const int* d_n_spans() const { return nspans_.as<int>(); }
     long long last_M() const { return last_M_; }
 
+    // Prefix beam search on the logits of the last forward (outputs on the
+    // device, as w2v_ctc_beam's); false: sizes that it does not take.
+    bool beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st);
+
     // Device error word set by kernels whose bounded waits expired.
     int check_device_error();
 
@@ -179,6 +183,8 @@ private:
     DevBuf logits_, ids_, spans_, nspans_;
     DevBuf err_;
     long long last_M_ = 0;
+    int last_n_utt_ = 0, last_T_max_ = 0;
+    DevBuf beam_state_;
     long long launches_cur_ = 0, launches_last_ = 0;
 
     // Captured forwards (CUDA graphs) of Engine::forward, keyed by the input
