@@ -210,6 +210,17 @@ def test_many_adapters_in_one_tile(K, synth, weights):
     c.check()
 
 
+@pytest.mark.parametrize("epi", [EPI_F16, EPI_F32, EPI_F32_RESID])
+@pytest.mark.parametrize("rank,n_adapters,N,lens", [(16, 12, 96, [1] * 40), (8, 15, 200, [3] * 50), (64, 3, 94, [1, 0, 200, 5, 77]),
+                                                     (128, 1, 40, [9, 130]), (24, 7, 64, [40] * 9), (72, 2, 1024, [1, 1, 1])])
+def test_lora_few_rows(K, synth, rank, n_adapters, N, lens, epi):
+    """A wave of tiles or less, both products in one kernel: adapters up to what the tile
+    holds, operand tiles in several batches, ranks that end inside a step of 16."""
+    c = Lora(K, synth, Segments(lens), [i * 5 % (n_adapters + 1) - 1 for i in range(len(lens))], N, 256, rank, n_adapters, "f16", epi)
+    c.call()
+    c.check()
+
+
 @pytest.mark.parametrize("weights", ["f16", "q8"])
 @pytest.mark.parametrize("n_utt,top", [(129, 3), (1500, 3), (400, 40), (3000, 2), (700, 0)])
 def test_many_utterances(K, synth, weights, n_utt, top):
@@ -392,3 +403,19 @@ def test_grouped_infinite_weights_of_other_groups(K):
                    seg.T.data_ptr(), gr.data_ptr(), 2, 0, st())
     torch.cuda.synchronize()
     assert torch.isfinite(out).all() and (out[3:5] == 0).all()
+
+
+def test_grouped_overlapping_utterances(K):
+    """Utterances that claim the same rows are not allowed for; a call that has many of them
+    ends, and stays within the rows."""
+    M, N, Kd, n = 300, 64, 128, 200
+    x, w = torch.randn(M, Kd, device="cuda").half(), (torch.randn(1, N, Kd, device="cuda") / Kd ** 0.5).half()
+    out = torch.full((M + 3, N), float("nan"), device="cuda")
+    off, T = torch.zeros(n, dtype=torch.int64, device="cuda"), torch.full((n,), M, dtype=torch.int32, device="cuda")
+    which, err = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    K.gemm_grouped(x.data_ptr(), Kd, Kd, M, w.data_ptr(), 1, N, out.data_ptr(), N, 0, 0, N, EPI_F32, off.data_ptr(), T.data_ptr(),
+                   which.data_ptr(), n, err.data_ptr(), st())
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0 and torch.isnan(out[M:]).all()
+    z, size = x.double() @ w[0].double().T, x.double().abs() @ w[0].double().abs().T
+    assert ((out[:M].double() - z).abs() <= (Kd / 16 + 8) * 2.0 ** -23 * size + 2.0 ** -24 * z.abs()).all()

@@ -56,7 +56,7 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
                                long long workspace_bytes, int* err, void* stream) {
     if (lda < K || lda % 8 || rank < 8 || rank > 128 || rank % 8 || n_adapters <= 0 || !lora_a || !lora_b ||
         ((reinterpret_cast<uintptr_t>(lora_a) | reinterpret_cast<uintptr_t>(lora_b)) & 15) || n_utt < 0 ||
-        epilogue == W2V_EPI_F32_RESID_LN || !Bq || !Bs || K > 0x7fffffffLL)
+        M > 0x7fffffffLL - 512 || N > 0x7fffffff - 512 || n_utt > 0x7fffffff - 512 || epilogue == W2V_EPI_F32_RESID_LN || !Bq || !Bs || K > 0x7fffffffLL)
         return W2V_ERR_ARGS;
     if (M == 0 && K > 0 && K % kBK == 0 && N > 0 && ldc >= N) return W2V_OK;
     if (n_utt > 0 && (!off || !T || !adapter)) return W2V_ERR_ARGS;

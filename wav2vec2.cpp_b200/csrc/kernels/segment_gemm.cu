@@ -55,7 +55,7 @@ __host__ __device__ constexpr int sum_blocks(int epi) { return epi == W2V_EPI_F3
 
 struct Params {
     int M, N, k_blocks;
-    int bn, n_tiles, m_tiles;                  // m_tiles: lora
+    int bn, n_tiles, m_tiles;                  // m_tiles, of rows: lora: all; grouped: no more than so many
     int stages, b_bytes;
     int vec, tma_c, bias_vec, bias_stride;     // wide stores; fp16 tile stores; wide bias loads; grouped: N
     void* C;
@@ -107,12 +107,12 @@ struct Walker {
         }
         total = __shfl_sync(0xffffffffu, incl, 31);
     }
-    // all row tiles of the batch
+    // all row tiles of the batch (utterances that overlap could have more than fit an int)
     W2V_DEV int count(const Params& p, int tile_rows) {
         int n = 0;
-        for (base = 0; base < p.n_utt; base += 32) {
+        for (base = 0; base < p.n_utt && n < p.m_tiles; base += 32) {
             load(p, tile_rows);
-            n += total;
+            n = min(n + total, p.m_tiles);
         }
         base = -32;
         total = 0;
@@ -637,8 +637,8 @@ struct Call {
 
 static bool refused(const Call& c) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(c.A), b = reinterpret_cast<uintptr_t>(c.B);
-    if (c.K <= 0 || c.K % 64 || c.K > 0x7fffffffLL || c.M < 0 || c.M > 0x7fffffffLL - 512 || c.N <= 0 || c.lda < c.K ||
-        c.lda % 8 || c.ldc < c.N || ((a | b) & 15) || c.epilogue < W2V_EPI_F16 || c.epilogue > W2V_EPI_F32_RESID ||
+    if (c.K <= 0 || c.K % 64 || c.K > 0x7fffffffLL || c.M < 0 || c.M > 0x7fffffffLL - 512 || c.N <= 0 || c.N > 0x7fffffff - 512 ||
+        c.n_utt > 0x7fffffff - 512 || c.lda < c.K || c.lda % 8 || c.ldc < c.N || ((a | b) & 15) || c.epilogue < W2V_EPI_F16 || c.epilogue > W2V_EPI_F32_RESID ||
         c.n_utt < 0)
         return true;
     return c.M > 0 && (!c.A || !c.B || !c.C || (c.epilogue == W2V_EPI_F32_RESID && (!c.resid || c.ldr < c.N)) ||
@@ -695,7 +695,7 @@ static int common(const Call& c, int bn, bool pair, Params& p, Maps& m) {
 using namespace w2v::sg;
 
 extern "C" long long w2v_lora_workspace_bytes(long long M, int n_utt, int rank) {
-    if (M < 0 || n_utt < 0 || rank < 8 || rank > 128 || rank % 8) return -1;
+    if (M < 0 || M > 0x7fffffffLL - 512 || n_utt < 0 || n_utt > 0x7fffffff - 512 || rank < 8 || rank > 128 || rank % 8) return -1;
     return lora_workspace(M, n_utt, rank);
 }
 
@@ -778,8 +778,9 @@ extern "C" int w2v_gemm_grouped_f16(const void* A, long long lda, long long K, l
     p.group = group;
     p.n_utt = n_utt;
     p.n_groups = n_groups;
-    const long long tiles = (M / (pair ? 256 : 128) + more) * p.n_tiles;
+    const long long m_tiles = M / (pair ? 256 : 128) + more, tiles = m_tiles * p.n_tiles;
     if (tiles > 0x7fffffffLL / 2) return W2V_ERR_ARGS;
+    p.m_tiles = (int)m_tiles;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return pair ? launch_epi<true, false>(epilogue, m, p, (int)tiles, false, st)
                 : launch_epi<false, false>(epilogue, m, p, (int)tiles, false, st);
