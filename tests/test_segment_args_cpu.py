@@ -94,3 +94,23 @@ def test_beam_state(L):
     assert beam(L, n_utt=0, logits=None, off=None, T=None, state=None, state_bytes=0) == OK
     for bad in ((-1, 32, 8, 100), (2, 1, 8, 100), (2, 1025, 8, 100), (2, 32, 0, 100), (2, 32, 129, 100), (2, 32, 8, 0), (2, 32, 128, 1 << 24)):
         assert L.w2v_ctc_beam_state_bytes(*bad) == -1
+
+
+HUGE = 0x7fffffff - 100          # sizes whose tiles an int could not number
+
+
+@pytest.mark.parametrize("f", [lora, lora_q, group])
+@pytest.mark.parametrize("bad", [dict(M=HUGE), dict(N=HUGE, ldc=HUGE, ld_s=HUGE + 7 & ~7), dict(n_utt=HUGE)])
+def test_sizes_near_the_end_of_an_int_are_refused(L, f, bad):
+    if f is not lora_q:
+        bad = {k: v for k, v in bad.items() if k != "ld_s"}
+    assert f(L, **bad, **({} if f is group else dict(ws_bytes=1 << 60))) == ARGS
+
+
+def test_bytes_that_pass_64_bits_are_refused(L):
+    assert L.w2v_lora_workspace_bytes(1 << 60, 3, 128) == -1 and L.w2v_lora_workspace_bytes(10, HUGE, 128) == -1
+    per = L.w2v_ctc_beam_state_bytes(1, 32, 128, 16000000)
+    n = 0x7fffffff
+    assert per > 0 and per * n > (1 << 63) - 1               # (a product of 64 bits would be another number)
+    assert L.w2v_ctc_beam_state_bytes(n, 32, 128, 16000000) == -1
+    assert beam(L, n_utt=n, width=128, max_frames=16000000, state_bytes=(1 << 63) - 1) == ARGS

@@ -808,7 +808,8 @@ extern "C" long long w2v_ctc_beam_state_bytes(int n_utt, int V, int width, int m
     if (n_utt < 0 || V < 2 || V > kMaxVocab || width < 1 || width > kMaxWidth || max_frames < 1 ||
         (long long)width * max_frames >= 0x7fffffffLL)
         return -1;
-    return n_utt * layout(width, max_frames).bytes;
+    const long long bytes = layout(width, max_frames).bytes;
+    return n_utt <= 0x7fffffffffffffffLL / bytes ? n_utt * bytes : -1;
 }
 
 extern "C" int w2v_ctc_beam(const float* logits, const long long* off, const int* T, int n_utt, int V, int blank,
