@@ -362,6 +362,36 @@ def test_beam_of_a_forward(K, pkg, model_path, synth):
     m.close()
 
 
+def test_beam_without_a_batch(K, pkg, model_path, synth):
+    """Before any forward, after one of no utterances and after one whose buffers did not fit there is
+    nothing to search; utterances without a frame have the empty hypothesis."""
+    import w2v_b200.binding as B
+    m = B.Model(model_path("tiny", "q8_0", bias_std=0.02, gain_jitter=0.1))
+    audio = torch.from_numpy(synth.make_audio(9000, 3)).cuda()
+    ids = torch.full((2, 1, 5), -7, dtype=torch.int32, device="cuda")
+    n_ids = torch.full((2, 1), -7, dtype=torch.int32, device="cuda")
+    scores = torch.full((2, 1), 7.0, dtype=torch.float64, device="cuda")
+
+    def search():
+        m.beam_device(4, 1, ids.data_ptr(), 5, n_ids.data_ptr(), scores.data_ptr())
+        torch.cuda.synchronize()
+        return n_ids.flatten().tolist(), scores.flatten().tolist()
+
+    untouched = [-7, -7], [7.0, 7.0]
+    assert search() == untouched
+    m.forward_device(audio.data_ptr(), [8000, 300])
+    assert search()[0][1] == 0
+    n_ids.fill_(-7), scores.fill_(7.0)
+    m.forward_device(audio.data_ptr(), [])
+    assert search() == untouched
+    with pytest.raises(B.EngineError):           # terabytes of activations: refused by the allocator, nothing is launched
+        m.forward_device(audio.data_ptr(), [0x7fffffff] * 4096)
+    assert search() == untouched
+    m.forward_device(audio.data_ptr(), [300, 20])
+    assert search() == ([0, 0], [0.0, 0.0]) and (ids == -1).all()
+    m.close()
+
+
 def test_adapters_heads_and_beams_together(K):
     """One batch of utterances in three languages: a shared projection with an adapter for
     each, an output head for each, and the beams over the logits; logits and hypotheses

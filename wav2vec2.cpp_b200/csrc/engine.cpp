@@ -15,7 +15,9 @@ namespace w2v {
 namespace {
 
 void cuda_check(cudaError_t e, const char* what) {
-    if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+    if (e == cudaSuccess) return;
+    cudaGetLastError();      // reported here: the next launch must not find it
+    throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 void w2v_check(int rc, const char* what) {
     if (rc != W2V_OK) {
@@ -542,12 +544,13 @@ int Engine::check_device_error() {
 bool Engine::fwd_begin(const BatchGeom& g, cudaStream_t st) {
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     last_M_ = g.M;
-    last_n_utt_ = g.n_utt;
+    last_n_utt_ = 0;                 // until the buffers hold this batch
     last_T_max_ = g.T_max;
     launches_cur_ = 0;
     if (g.n_utt == 0) { launches_last_ = 0; return false; }
     ensure_workspace(g);
     upload_meta(g, st);
+    last_n_utt_ = g.n_utt;
     if (g.M == 0) {
         cuda_check(cudaMemsetAsync(nspans_.p, 0, sizeof(int) * g.n_utt, st), "memset");
         launches_last_ = 0;
