@@ -248,6 +248,18 @@ def test_large_batch_uses_all_row_blocks(K, synth, weights):
     c.check()
 
 
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 64, 72, 104, 128])
+@pytest.mark.parametrize("Kd", [64, 192, 1088])
+@pytest.mark.parametrize("lens,n_adapters", [([70, 1, 40], 3), ([30] * 12, 12), ([1000] * 18 + [500, 700], 5)])
+def test_ranks_and_depths(K, synth, rank, Kd, lens, n_adapters):
+    """Fewer steps of K than the first product has stages and warps, and several rounds of its
+    stages; each adapter with blocks of its own (few rows), or two and more in turn."""
+    c = Lora(K, synth, Segments(lens), [(5 * i + 1) % n_adapters for i in range(len(lens))], 64, Kd, rank, n_adapters, "f16", EPI_F32)
+    c.call()
+    c.call()
+    c.check()
+
+
 @pytest.mark.parametrize("weights,epi", [("f16", EPI_F16), ("f16", EPI_F32), ("q8", EPI_F16), ("q8", EPI_F32)])
 def test_strides_and_missing_operands(K, synth, weights, epi):
     """Rows of A and C further apart than their widths, no bias, no scale."""

@@ -21,11 +21,14 @@ namespace w2v {
 namespace sg {
 
 constexpr int kStep = 64, kMaxTile = 256;
-constexpr int kPlanners = 128, kThreads = kPlanners + 32;
+constexpr int kPlanners = 128, kProducer = kPlanners / 32, kIssuers = 4, kThreads = kPlanners + 32 + 32 * kIssuers;
 constexpr int kMaxRing = 8;
+constexpr int kDirect = 64;
 
 struct ShrinkShape {
     int stages, stage_bytes, smem, cols;       // cols: of TMEM
+    int issuers;                               // warps that multiply
+    int direct;                                // block y takes adapter y, used or not
 };
 // Two blocks per SM where a ring of three stages or more allows it.
 static ShrinkShape shrink_shape(int rows, int rank) {
@@ -35,9 +38,13 @@ static ShrinkShape shrink_shape(int rows, int rank) {
     const int two = (108 * 1024 - behind) / s.stage_bytes, one = (216 * 1024 - behind) / s.stage_bytes;
     s.stages = two >= 3 ? two : one;
     if (s.stages > kMaxRing) s.stages = kMaxRing;
+    if (s.stages > 3) s.stages &= ~1;
     s.smem = 1024 + s.stages * s.stage_bytes + behind + 256;
+    const int acc = 2 * ((rank + 15) / 16 * 16);
+    s.issuers = kIssuers;
+    while (s.issuers > 1 && (s.issuers * acc > 256 || s.stages % s.issuers)) s.issuers /= 2;
     s.cols = 32;
-    while (s.cols < 2 * ((rank + 15) / 16 * 16)) s.cols *= 2;
+    while (s.cols < s.issuers * acc) s.cols *= 2;
     return s;
 }
 
@@ -69,8 +76,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     __shared__ int counts[kPlanners / 32];
     __shared__ int row_slot[128];             // of this block's rows
     __shared__ int n_here_shared;
-    __shared__ long long first_block_shared;
-    __shared__ uint64_t full[kMaxRing], empty[kMaxRing], done;
+    __shared__ uint64_t full[kMaxRing], empty[kMaxRing], done, drained;
     __shared__ uint32_t tmem_slot;
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* ring = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -84,8 +90,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const int local0 = (int)(row0 - tile0);
     const int k_steps = a.K / kStep;
     const long long part = p.blocks * p.tile * rank;
+    const bool direct = shape.direct != 0;
     // the block that is sure to use its rows fetches the first of them before it knows the adapters
-    const int early = blockIdx.y == 0 ? min(S, k_steps) : 0;
+    const int early = blockIdx.y == 0 && !direct ? min(S, k_steps) : 0;
+    const int issuers = shape.issuers, acc_cols = 2 * n16;
 
     // a stage's x and the adapters' share complete on full[st]
     const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), lead = elect_one();
@@ -93,10 +101,59 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         tma_load_2d_if<false>(lead, ring0 + (uint32_t)(st * shape.stage_bytes), &tmX, full0 + (uint32_t)(st * 8), ks * kStep,
                               (int)row0);
     };
-    if (warp == kPlanners / 32) {
+    int st = 0, used = 0;                     // the producer's: its stage, and stages filled so far
+    uint32_t odd = 0, issued = 0;
+    bool ok = true;
+    auto fill = [&](int n, int ad0, int ad1) {        // x and n adapters' A
+        for (int ks = 0; ks < k_steps; ks++) {
+            if (used >= S && !mbar_wait_warp(&empty[st], odd ^ 1u, a.err)) { ok = false; break; }
+            const uint32_t sa = ring0 + (uint32_t)(st * shape.stage_bytes + kXBytes), bar = full0 + (uint32_t)(st * 8);
+            expect_tx_if(lead, bar, (uint32_t)(n * a_bytes + (used >= early ? kXBytes : 0)));
+            tma_load_3d_if<false>(lead, sa, &tmA, bar, ks * kStep, 0, ad0);
+            if (n > 1) tma_load_3d_if<false>(lead, sa + (uint32_t)a_bytes, &tmA, bar, ks * kStep, 0, ad1);
+            if (used >= early) load_x(st, ks);
+            issued |= 1u << st;
+            used++;
+            if (++st == S) { st = 0; odd ^= 1u; }
+        }
+    };
+    // K-steps w, w + issuers, .. of a pass into issuer w's own accumulators; the pass begins at stage `st`.
+    // The ring is a multiple of the issuers, so that a stage is always the same one's: another could look
+    // for its second filling while the first is on its way, and take the phase before for it.
+    auto multiply = [&](int n, int pass) {
+        const int w = warp - kProducer - 1;
+        if (w >= issuers) return;
+        if (pass > 0 && ok && !mbar_wait_warp(&drained, (uint32_t)(pass - 1) & 1u, a.err)) ok = false;
+        tc_fence_after();
+        const uint32_t idesc = umma_idesc_f16(128, n16), d0 = (uint32_t)uniform((int)tmem_slot) + (uint32_t)(w * acc_cols);
+        const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
+        int at = st + w;
+        uint32_t par = odd;
+        if (at >= S) { at -= S; par ^= 1u; }
+        for (int ks = w; ks < k_steps && ok; ks += issuers) {
+            if (!mbar_wait_warp(&full[at], par, a.err)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t dx = desc_plus(desc0, (uint32_t)(at * shape.stage_bytes));
+            for (int e = 0; e < n; e++) {
+                const uint64_t db = desc_plus(dx, (uint32_t)(kXBytes + e * a_bytes));
+                const uint32_t d = d0 + (uint32_t)(e * n16);
+#pragma unroll
+                for (int kk = 0; kk < kStep / 16; kk++)
+                    umma_f16_if<false>(lead, d, desc_plus(dx, kk * 32), desc_plus(db, kk * 32), idesc, ks != w || kk != 0);
+            }
+            umma_commit_if<false>(lead, smem_u32(&empty[at]));
+            at += issuers;
+            if (at >= S) { at -= S; par ^= 1u; }
+        }
+        umma_commit_if<false>(lead, smem_u32(&done));     // (also after an expired wait)
+        odd ^= (uint32_t)((st + k_steps) / S) & 1u;
+        st = (st + k_steps) % S;
+    };
+    if (warp == kProducer) {
         if (lane == 0) {
             for (int s = 0; s < S; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-            mbar_init(&done, 1);
+            mbar_init(&done, issuers);
+            mbar_init(&drained, kPlanners / 32);
             fence_mbar_init();
         }
         __syncwarp();
@@ -105,15 +162,26 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             load_x(ks, ks);
         }
     }
-    if (warp == 0) {
+    if (warp == kProducer + 1) {
         // TMEM first: a projection's block that came to this SM before would hold all of it
         // while it waits for this grid
         tmem_alloc(&tmem_slot, shape.cols);
         tmem_relinquish();
         grid_launch_dependents();
     }
+    if (warp >= kProducer) {                  // the planners need neither barriers nor TMEM yet
+        tc_fence_before();
+        asm volatile("barrier.sync 2, %0;" ::"n"(kThreads - kPlanners) : "memory");
+        tc_fence_after();
+        if (direct) {
+            if (warp == kProducer) fill(1, (int)blockIdx.y, 0);
+            else multiply(1, 0);
+        }
+    }
 
-    if (warp < kPlanners / 32) {
+    int n_here = 0, count = 0;
+    long long first_block = 0;
+    if (warp < kProducer) {
         if (tid == 0) present_mask = 0;
         auto end_of = [&](int u) { return a.off[u] + max(a.T[u], 0); };
 
@@ -161,8 +229,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             if (u0 + kPlanners < a.n_utt && plan_count(past)) break;
         }
         n_seg = min(n_seg, kMaxTile);
-        const long long first_block = tile + (ended < tile0 ? ended : tile0);
-        int count = 0, n_here = 0;
+        first_block = tile + (ended < tile0 ? ended : tile0);
         if (n_seg <= 32) {
             // by every warp for itself: each adapter once, and the row's
             const int v = lane < n_seg ? seg_adapter[lane] : -1;
@@ -262,7 +329,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                 p.adapter[first_block + i] = slots[i];
             }
         }
-        if (blockIdx.y == 0)                      // the others' blocks are zero in these rows
+        if (blockIdx.y == 0 && !direct)           // the others' blocks are zero in these rows
             for (int k = n_here; k < count; k++) {
                 __half* out = p.t + ((first_block + here[k]) * p.tile + local0) * rank;
                 const int n = min(kRows, n_rows - local0) * rank / 8;
@@ -271,35 +338,20 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     if (p.parts == 2) reinterpret_cast<uint4*>(out + part)[c] = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
-        if (tid == 0) { n_here_shared = n_here; first_block_shared = first_block; }
+        if (tid == 0) n_here_shared = n_here;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const int n_here = n_here_shared;
-    const long long first_block = first_block_shared;
+    n_here = n_here_shared;
 
-    // adapters of a pass: two, or one where there are blocks for each; the ring's counters run on
-    const int side = n_here > (int)gridDim.y ? 2 : 1;
-    const uint32_t tmem = (uint32_t)uniform((int)tmem_slot);
-    if (warp == kPlanners / 32) {
-        int st = 0, used = 0;                 // used: stages filled so far
-        uint32_t odd = 0, issued = 0;
-        bool ok = true;
-        for (int base = side * blockIdx.y; base < n_here && ok; base += side * gridDim.y) {
+    // adapters of a pass: two, or one where there are blocks for each
+    const int side = n_here > (int)gridDim.y ? 2 : 1, stride = side * (int)gridDim.y, base0 = side * (int)blockIdx.y;
+    if (warp == kProducer) {
+        for (int base = base0; base < n_here && ok && !direct; base += stride) {
             const int n = uniform(min(side, n_here - base));
             const int ad0 = uniform(slots[here[base]]), ad1 = uniform(n > 1 ? slots[here[base + 1]] : 0);
-            for (int ks = 0; ks < k_steps; ks++) {
-                if (used >= S && !mbar_wait_warp(&empty[st], odd ^ 1u, a.err)) { ok = false; break; }
-                const uint32_t sa = ring0 + (uint32_t)(st * shape.stage_bytes + kXBytes), bar = full0 + (uint32_t)(st * 8);
-                expect_tx_if(lead, bar, (uint32_t)(n * a_bytes + (used >= early ? kXBytes : 0)));
-                tma_load_3d_if<false>(lead, sa, &tmA, bar, ks * kStep, 0, ad0);
-                if (n > 1) tma_load_3d_if<false>(lead, sa + (uint32_t)a_bytes, &tmA, bar, ks * kStep, 0, ad1);
-                if (used >= early) load_x(st, ks);
-                issued |= 1u << st;
-                used++;
-                if (++st == S) { st = 0; odd ^= 1u; }
-            }
+            fill(n, ad0, ad1);
         }
         // no bulk copy may still be writing shared memory when the block exits: rows that
         // no adapter came for, and what the MMAs have not waited for
@@ -310,74 +362,75 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         for (int s = 0; s < S; s++)
             if (issued >> s & 1u) mbar_wait(&full[s], s < st ? odd : odd ^ 1u, a.err);
         __syncwarp();
+    } else if (warp > kProducer) {
+        int pass = 0;
+        for (int base = base0; base < n_here && !direct; base += stride, pass++) multiply(min(side, n_here - base), pass);
     } else {
-        int st = 0, pass = 0;
-        uint32_t odd = 0;
-        bool ok = true;
-        for (int base = side * blockIdx.y; base < n_here; base += side * gridDim.y, pass++) {
-            const int n = min(side, n_here - base);
-            if (warp == 0) {
-                const uint32_t idesc = umma_idesc_f16(128, n16);
-                const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
-                for (int ks = 0; ks < k_steps && ok; ks++) {
-                    if (!mbar_wait_warp(&full[st], odd, a.err)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint64_t dx = desc_plus(desc0, (uint32_t)(st * shape.stage_bytes));
-                    for (int e = 0; e < n; e++) {
-                        const uint64_t db = desc_plus(dx, (uint32_t)(kXBytes + e * a_bytes));
-                        const uint32_t d = tmem + (uint32_t)(e * n16);
+        const uint32_t tmem = (uint32_t)uniform((int)tmem_slot);
+        const int parts = min(issuers, k_steps);
+        // an adapter's share, masked, as fp16 (and what the rounding left, for fp32 outputs): a row per lane
+        const int r = warp * 32 + lane;
+        const bool real = local0 + r < n_rows;
+        const int mine = row_slot[r];
+        auto store = [&](int e, int s) {
+            const float sc = a.scale ? a.scale[slots[s]] : 1.f;
+            __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * rank;
+            for (int c = 0; c < rank; c += 16) {
+                const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * n16 + c);
+                float v[16];
+                tmem_ld16(from, v);
+                for (int w = 1; w < parts; w++) {
+                    float x[16];
+                    tmem_ld16(from + (uint32_t)(w * acc_cols), x);
 #pragma unroll
-                        for (int kk = 0; kk < kStep / 16; kk++)
-                            umma_f16_if<false>(lead, d, desc_plus(dx, kk * 32), desc_plus(db, kk * 32), idesc,
-                                               (ks | kk) != 0);
-                    }
-                    umma_commit_if<false>(lead, smem_u32(&empty[st]));
-                    if (++st == S) { st = 0; odd ^= 1u; }
+                    for (int i = 0; i < 16; i++) v[i] += x[i];
                 }
-                umma_commit_if<false>(lead, smem_u32(&done));     // (also after an expired wait)
+                uint32_t hi[8], low[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float v0 = mine == s ? v[2 * i] * sc : 0.f, v1 = mine == s ? v[2 * i + 1] * sc : 0.f;
+                    const __half2 h = __floats2half2_rn(v0, v1);
+                    const float2 f = __half22float2(h);
+                    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    low[i] = pack_half2(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
+                }
+                if (!real) continue;
+                uint4* o = reinterpret_cast<uint4*>(out + c);
+                uint4* o2 = reinterpret_cast<uint4*>(out + part + c);
+                o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (p.parts == 2) o2[0] = make_uint4(low[0], low[1], low[2], low[3]);
+                if (c + 16 <= rank) {
+                    o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                    if (p.parts == 2) o2[1] = make_uint4(low[4], low[5], low[6], low[7]);
+                }
             }
+        };
+        if (direct) {
+            int s = 0;                        // this block's adapter among the tile's
+            while (s < count && slots[s] != (int)blockIdx.y) s++;
+            mbar_wait(&done, 0, a.err);
+            __syncwarp();
+            tc_fence_after();
+            if (s < count && warp * 32 < kRows) store(0, s);
+        }
+        int pass = 0;
+        for (int base = base0; base < n_here && !direct; base += stride, pass++) {
             mbar_wait(&done, (uint32_t)pass & 1u, a.err);
+            __syncwarp();
             tc_fence_after();
-            // masked, as fp16 (and what the rounding left, for fp32 outputs): a row per lane
-            const int r = warp * 32 + lane;
-            if (warp * 32 < kRows) {
-                const bool real = local0 + r < n_rows;
-                const int mine = row_slot[r];
-                for (int e = 0; e < n; e++) {
-                    const int s = here[base + e];
-                    const float sc = a.scale ? a.scale[slots[s]] : 1.f;
-                    __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * rank;
-                    for (int c = 0; c < rank; c += 16) {
-                        float v[16];
-                        tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * n16 + c), v);
-                        uint32_t hi[8], low[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float v0 = mine == s ? v[2 * i] * sc : 0.f, v1 = mine == s ? v[2 * i + 1] * sc : 0.f;
-                            const __half2 h = __floats2half2_rn(v0, v1);
-                            const float2 f = __half22float2(h);
-                            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-                            low[i] = pack_half2(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
-                        }
-                        if (!real) continue;
-                        uint4* o = reinterpret_cast<uint4*>(out + c);
-                        uint4* o2 = reinterpret_cast<uint4*>(out + part + c);
-                        o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        if (p.parts == 2) o2[0] = make_uint4(low[0], low[1], low[2], low[3]);
-                        if (c + 16 <= rank) {
-                            o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                            if (p.parts == 2) o2[1] = make_uint4(low[4], low[5], low[6], low[7]);
-                        }
-                    }
-                }
-            }
-            tc_fence_before();
-            plan_sync();                      // the accumulators are read before the next pass's products
-            tc_fence_after();
+            if (warp * 32 < kRows)
+                for (int e = 0; e < min(side, n_here - base); e++) store(e, here[base + e]);
+            tc_fence_before();                // the accumulators are read before the next pass's products
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&drained);
         }
     }
+    tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, shape.cols);
+    if (warp == kProducer + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_slot, shape.cols);
+    }
 }
 
 template <int ROWS>
@@ -407,7 +460,9 @@ static int launch_rows(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
     long long ny = 296 / chunks;
     if (ny > most) ny = most;
     if (ny < 1) ny = 1;
-    const ShrinkShape shape = shrink_shape(ROWS, p.rank);
+    ShrinkShape shape = shrink_shape(ROWS, p.rank);
+    shape.direct = chunks * a.n_adapters <= kDirect;
+    if (shape.direct) ny = a.n_adapters;
     kern<<<dim3((unsigned)chunks, (unsigned)ny), kThreads, shape.smem, st>>>(tx, ta, a, p, shape);
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
