@@ -412,30 +412,44 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             for (int tile = unit; tile < total && ok; tile += n_units) {
                 bool first = true;               // stage of a sum
                 uint32_t d = 0;
-                for (int kb = 0; WORK || kb < p.k_blocks; kb++) {
+                // a stage's operands are there, and an accumulator for the first of a sum
+                auto begin = [&] {
                     if (first) {
-                        if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1u, p.err)) { ok = false; break; }
+                        if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1u, p.err)) return false;
                         d = accumulator_at(acc);
                     }
-                    if (!mbar_wait_warp(&full[stage], phase, p.err)) { ok = false; break; }
+                    if (!mbar_wait_warp(&full[stage], phase, p.err)) return false;
                     tc_fence_after();
-                    const uint32_t work = WORK ? (uint32_t)uniform((int)stage_work[stage])
-                                               : kBK / 16 | (kb == p.k_blocks - 1 ? kLastOfSum : 0);
+                    return true;
+                };
+                auto multiply = [&](uint32_t go, int kk) {
                     const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
-#pragma unroll
-                    for (uint32_t kk = 0; kk < kBK / 16; kk++)
-                        umma_f16_if<PAIR>(LORA ? lead & (uint32_t)(kk < (work & 15u)) : lead, d, desc_plus(da, kk * 32),
-                                          desc_plus(db, kk * 32), idesc, !first || kk != 0);
+                    umma_f16_if<PAIR>(go, d, desc_plus(da, kk * 32), desc_plus(db, kk * 32), idesc, !first || kk != 0);
+                };
+                auto end = [&](bool last_of_sum) {
                     umma_commit_if<PAIR>(lead, empty_here + (uint32_t)(stage * 8));
                     if (PAIR) umma_commit_if<PAIR>(lead, empty_peer + (uint32_t)(stage * 8));
                     if (++stage == S) { stage = 0; phase ^= 1u; }
-                    first = (work & kLastOfSum) != 0;
-                    if (first) {
+                    first = last_of_sum;
+                    if (last_of_sum) {
                         umma_commit_if<PAIR>(lead, tfull_here + acc * 8u);
                         if (PAIR) umma_commit_if<PAIR>(lead, tfull_peer + acc * 8u);
                         if (++acc == n_acc) { acc = 0; acc_phase ^= 1u; }
                     }
-                    if (WORK && (work & kLastOfTile)) break;
+                };
+                for (int kb = 0; kb < p.k_blocks - 1; kb++) {
+                    if (!begin()) { ok = false; break; }
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; kk++) multiply(lead, kk);
+                    end(SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1);
+                }
+                // the last of K and the adapters' stages: as the producer found them
+                for (uint32_t work = 0; ok && !(work & kLastOfTile);) {
+                    if (!begin()) { ok = false; break; }
+                    work = WORK ? (uint32_t)uniform((int)stage_work[stage]) : kBK / 16 | kLastOfSum | kLastOfTile;
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; kk++) multiply(LORA ? lead & (uint32_t)(kk < (int)(work & 15u)) : lead, kk);
+                    end((work & kLastOfSum) != 0);
                 }
             }
             // no MMA may still be writing TMEM when it is freed (also after an expired wait)
