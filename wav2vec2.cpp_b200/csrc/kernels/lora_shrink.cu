@@ -23,12 +23,13 @@ namespace sg {
 constexpr int kStep = 64, kMaxTile = 256;
 constexpr int kPlanners = 128, kProducer = kPlanners / 32, kIssuers = 4, kThreads = kPlanners + 32 + 32 * kIssuers;
 constexpr int kMaxRing = 8;
-constexpr int kDirect = 64;
+constexpr int kDirect = 32;
 
 struct ShrinkShape {
     int stages, stage_bytes, smem, cols;       // cols: of TMEM
     int issuers;                               // warps that multiply
     int direct;                                // block y takes adapter y, used or not
+    int x_bytes;                               // of a box of x
 };
 // Two blocks per SM where a ring of three stages or more allows it.
 static ShrinkShape shrink_shape(int rows, int rank) {
@@ -108,7 +109,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         for (int ks = 0; ks < k_steps; ks++) {
             if (used >= S && !mbar_wait_warp(&empty[st], odd ^ 1u, a.err)) { ok = false; break; }
             const uint32_t sa = ring0 + (uint32_t)(st * shape.stage_bytes + kXBytes), bar = full0 + (uint32_t)(st * 8);
-            expect_tx_if(lead, bar, (uint32_t)(n * a_bytes + (used >= early ? kXBytes : 0)));
+            expect_tx_if(lead, bar, (uint32_t)(n * a_bytes + (used >= early ? shape.x_bytes : 0)));
             tma_load_3d_if<false>(lead, sa, &tmA, bar, ks * kStep, 0, ad0);
             if (n > 1) tma_load_3d_if<false>(lead, sa + (uint32_t)a_bytes, &tmA, bar, ks * kStep, 0, ad1);
             if (used >= early) load_x(st, ks);
@@ -158,7 +159,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         }
         __syncwarp();
         for (int ks = 0; ks < early; ks++) {
-            expect_more_if(lead, full0 + (uint32_t)(ks * 8), kXBytes);
+            expect_more_if(lead, full0 + (uint32_t)(ks * 8), (uint32_t)shape.x_bytes);
             load_x(ks, ks);
         }
     }
@@ -434,7 +435,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 }
 
 template <int ROWS>
-static int launch_rows(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
+static int launch_rows(const LoraArgs& a, const LoraPlan& p, const CUtensorMap* x, int x_rows, cudaStream_t st) {
     auto kern = lora_shrink_kernel<ROWS>;
     static bool attr_set[64] = {};
     int dev = 0;
@@ -446,7 +447,13 @@ static int launch_rows(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
     }
     CUtensorMap tx, ta;
     const uint64_t xd[2] = {(uint64_t)a.K, (uint64_t)a.M}, xs[1] = {(uint64_t)a.lda * 2};
-    int rc = map_f16(&tx, a.x, 2, xd, xs, ROWS);
+    int rc = W2V_OK;
+    if (x && (x_rows == ROWS || (x_rows < ROWS && a.M <= x_rows))) {
+        tx = *x;                               // (a box may be lower than a block that has no more rows)
+    } else {
+        x_rows = ROWS;
+        rc = map_f16(&tx, a.x, 2, xd, xs, ROWS);
+    }
     if (rc) return rc;
     const uint64_t ad[3] = {(uint64_t)a.K, (uint64_t)p.rank, (uint64_t)a.n_adapters};
     const uint64_t as[2] = {(uint64_t)a.K * 2, (uint64_t)a.K * 2 * p.rank};
@@ -461,14 +468,15 @@ static int launch_rows(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
     if (ny > most) ny = most;
     if (ny < 1) ny = 1;
     ShrinkShape shape = shrink_shape(ROWS, p.rank);
+    shape.x_bytes = x_rows * kStep * 2;
     shape.direct = chunks * a.n_adapters <= kDirect;
     if (shape.direct) ny = a.n_adapters;
     kern<<<dim3((unsigned)chunks, (unsigned)ny), kThreads, shape.smem, st>>>(tx, ta, a, p, shape);
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
 
-int lora_shrink(const LoraArgs& a, const LoraPlan& p, cudaStream_t st) {
-    return p.tile % 128 == 0 && a.M >= 128 * 148 ? launch_rows<128>(a, p, st) : launch_rows<64>(a, p, st);
+int lora_shrink(const LoraArgs& a, const LoraPlan& p, const CUtensorMap* x, int x_rows, cudaStream_t st) {
+    return p.tile % 128 == 0 && a.M >= 128 * 148 ? launch_rows<128>(a, p, x, x_rows, st) : launch_rows<64>(a, p, x, x_rows, st);
 }
 
 }  // namespace sg

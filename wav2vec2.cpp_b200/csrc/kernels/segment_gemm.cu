@@ -57,6 +57,7 @@ struct Params {
     int M, N, k_blocks;
     int bn, n_tiles, m_tiles;                  // m_tiles, of rows: lora: all; grouped: no more than so many
     int stages, b_bytes;
+    int a_rows;                                // rows of a stage's operand box: 128, lora: fewer where there are no more
     int vec, tma_c, bias_vec, bias_stride;     // wide stores; fp16 tile stores; wide bias loads; grouped: N
     void* C;
     long long ldc;
@@ -273,8 +274,7 @@ template <int EPI, bool PAIR, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1)
 seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmT,
-                const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmA32,
-                const __grid_constant__ CUtensorMap tmT32, const __grid_constant__ Params p) {
+                const __grid_constant__ CUtensorMap tmL, const __grid_constant__ Params p) {
     constexpr int CT = PAIR ? 2 : 1, kTileRows = kBM * CT;
     constexpr bool SUMS = sums_of(EPI), WORK = LORA || SUMS;   // WORK: a stage says what is to be done with it
     extern __shared__ uint8_t smem_raw[];
@@ -342,21 +342,20 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         uint32_t phase = 0, issued = 0, last_par = 0;
         bool ok = true;
         // one stage's two tiles; work: its MMA steps, and whether it is the last of a sum and of the tile
-        // of the rows only the 32-row boxes that hold valid ones, where that saves any: what the MMA
-        // reads in the others' places goes to accumulator rows that are not stored
+        // grouped: of the rows only the 32-row boxes that hold valid ones, where that saves any (tmT, which is
+        // theirs then): what the MMA reads in the others' places goes to accumulator rows that are not stored
         int boxes = 4;
-        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* ma32, const CUtensorMap* mb, int k, int ra, int rb, int gb,
-                            uint32_t work) {
+        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int k, int ra, int rb, int gb, uint32_t work) {
             if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
             const uint32_t dst = base + (uint32_t)(stage * stage_bytes), bar = full_lead + (uint32_t)(stage * 8);
             if (WORK && lane == 0) stage_work[stage] = work;
             if (WORK) __syncwarp();
             expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
-            if (boxes == 4) {
+            if (LORA || boxes == 4) {
                 tma_load_2d_if<PAIR>(lead, dst, ma, bar, k, ra + (int)rank * kBM);
             } else {
                 for (int i = 0; i < boxes; i++)
-                    tma_load_2d_if<PAIR>(lead, dst + (uint32_t)(i * kABytes / 4), ma32, bar, k, ra + (int)rank * kBM + i * 32);
+                    tma_load_2d_if<PAIR>(lead, dst + (uint32_t)(i * kABytes / 4), &tmT, bar, k, ra + (int)rank * kBM + i * 32);
             }
             tma_load_3d_if<PAIR>(lead, dst + kABytes, mb, bar, k, rb + b_row, gb);
             issued |= 1u << stage;
@@ -366,11 +365,15 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         for (int tile = unit; tile < total && ok; tile += n_units) {
             const Tile t = tile_at(tile);
             const int col0 = t.ni * p.bn;
-            auto boxes_of = [&](int r) { return max(min((t.end - r + 31) / 32, 4), 0); };
-            boxes = boxes_of(t.row0 + (int)rank * kBM);
-            arm_bytes = (uint32_t)(CT * p.b_bytes + (boxes_of(t.row0) + (PAIR ? boxes_of(t.row0 + kBM) : 0)) * (kABytes / 4));
+            if constexpr (LORA) {
+                arm_bytes = (uint32_t)(CT * (p.b_bytes + p.a_rows * kBK * 2));
+            } else {
+                auto boxes_of = [&](int r) { return max(min((t.end - r + 31) / 32, 4), 0); };
+                boxes = boxes_of(t.row0 + (int)rank * kBM);
+                arm_bytes = (uint32_t)(CT * p.b_bytes + (boxes_of(t.row0) + (PAIR ? boxes_of(t.row0 + kBM) : 0)) * (kABytes / 4));
+            }
             for (int kb = 0; kb < p.k_blocks - 1 && ok; kb++)
-                stage_in(&tmA, &tmA32, &tmB, kb * kBK, t.row0, col0, t.group,
+                stage_in(&tmA, &tmB, kb * kBK, t.row0, col0, t.group,
                          kBK / 16 | (SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1 ? kLastOfSum : 0));
             int blocks = 0, first = 0, rec = 0;
             if (LORA && p.lora) {
@@ -381,7 +384,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 blocks = uniform(__shfl_sync(0xffffffffu, rec, 1));
             }
             if (ok)
-                stage_in(&tmA, &tmA32, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile | kLastOfSum));
+                stage_in(&tmA, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile | kLastOfSum));
             for (int b = 0; b < blocks && ok; b++) {
                 const int held = __shfl_sync(0xffffffffu, rec, min(2 + b, 31));
                 const int ad = uniform(b < kInline ? held : p.plan.adapter[first + b]);
@@ -389,7 +392,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     const int trow = (int)((part * p.plan.blocks + first + b) * kTileRows);
                     for (int c = 0; c < chunks && ok; c++) {
                         const bool last = b + 1 == blocks && part + 1 == p.plan.parts && c + 1 == chunks;
-                        stage_in(&tmT, &tmT32, &tmL, c * kBK, trow, col0, ad,
+                        stage_in(&tmT, &tmL, c * kBK, trow, col0, ad,
                                  min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16) | (last ? kLastOfTile | kLastOfSum : 0));
                     }
                 }
@@ -554,7 +557,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 // ── host side ───────────────────────────────────────────────────────────────
 
 struct Maps {
-    CUtensorMap a, b, c, t, l, a32, t32;
+    CUtensorMap a, b, c, t, l;
 };
 
 template <int EPI, bool PAIR, bool LORA>
@@ -598,7 +601,7 @@ static int launch(const Maps& m, const Params& p, int tiles, bool dependent, cud
         attr[n].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = ++n;
     }
-    if (cudaLaunchKernelEx(&cfg, kern, m.a, m.b, m.c, m.t, m.l, m.a32, m.t32, p) != cudaSuccess) return W2V_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kern, m.a, m.b, m.c, m.t, m.l, p) != cudaSuccess) return W2V_ERR_LAUNCH;
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;
 }
 
@@ -660,7 +663,7 @@ static bool refused(const Call& c) {
 }
 
 // Parameters and maps that both products share.
-static int common(const Call& c, int bn, bool pair, Params& p, Maps& m) {
+static int common(const Call& c, bool lora, int bn, bool pair, Params& p, Maps& m) {
     const bool f16 = c.epilogue == W2V_EPI_F16 || c.epilogue == W2V_EPI_F16_GELU;
     const uintptr_t C = reinterpret_cast<uintptr_t>(c.C), R = reinterpret_cast<uintptr_t>(c.resid);
     p.M = (int)c.M;
@@ -681,14 +684,16 @@ static int common(const Call& c, int bn, bool pair, Params& p, Maps& m) {
     p.ldr = c.ldr;
     p.err = c.err;
     const uint64_t ad[2] = {(uint64_t)c.K, (uint64_t)c.M}, as[1] = {(uint64_t)c.lda * 2};
-    int rc = map_f16(&m.a, c.A, 2, ad, as, kBM);
-    if (!rc) rc = map_f16(&m.a32, c.A, 2, ad, as, 32);
+    p.a_rows = lora && c.M < kBM ? (int)((c.M + 31) / 32 * 32) : kBM;
+    int rc = map_f16(&m.a, c.A, 2, ad, as, p.a_rows);
+    if (rc) return rc;
+    m.c = m.t = m.l = m.a;
+    if (!lora) rc = map_f16(&m.t, c.A, 2, ad, as, 32);
     if (rc) return rc;
     const uint64_t bd[3] = {(uint64_t)c.K, (uint64_t)c.N, (uint64_t)c.n_mats};
     const uint64_t bs[2] = {(uint64_t)c.K * 2, (uint64_t)c.K * 2 * c.N};
     rc = map_f16(&m.b, c.B, 3, bd, bs, pair ? bn / 2 : bn);
     if (rc) return rc;
-    m.c = m.t = m.l = m.t32 = m.a;
     // fp16 C by 32 x 32 boxes; a store clips the innermost dimension at 16-byte granularity only
     p.tma_c = f16 && c.ldc % 8 == 0 && c.N % 8 == 0 && C % 16 == 0;
     if (p.tma_c) {
@@ -731,7 +736,7 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
     int bn = 256;
     bool pair = false;
     pick_tile(N, (M + 127) / 128, (M + 255) / 256, K, &bn, &pair);
-    int rc = common(c, bn, pair, p, m);
+    int rc = common(c, true, bn, pair, p, m);
     if (rc) return rc;
     const int tile_rows = pair ? 256 : 128;
     p.m_tiles = (int)((M + tile_rows - 1) / tile_rows);
@@ -741,8 +746,7 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
         if (p.plan.parts * p.plan.blocks * tile_rows > 0x7fffffffLL) return W2V_ERR_ARGS;
         const uint64_t td[2] = {(uint64_t)rank, (uint64_t)(p.plan.parts * p.plan.blocks * tile_rows)};
         const uint64_t ts[1] = {(uint64_t)rank * 2};
-        rc = map_f16(&m.t, p.plan.t, 2, td, ts, kBM);
-        if (!rc) rc = map_f16(&m.t32, p.plan.t, 2, td, ts, 32);
+        rc = map_f16(&m.t, p.plan.t, 2, td, ts, p.a_rows);
         if (rc) return rc;
         const uint64_t ld[3] = {(uint64_t)rank, (uint64_t)N, (uint64_t)n_adapters};
         const uint64_t ls[2] = {(uint64_t)rank * 2, (uint64_t)rank * 2 * N};
@@ -761,7 +765,7 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
         a.adapter = adapter;
         a.n_utt = n_utt;
         a.err = err;
-        rc = lora_shrink(a, p.plan, st);
+        rc = lora_shrink(a, p.plan, &m.a, p.a_rows, st);
         if (rc) return rc;
     }
     const long long tiles = (long long)p.m_tiles * p.n_tiles;
@@ -785,7 +789,7 @@ extern "C" int w2v_gemm_grouped_f16(const void* A, long long lda, long long K, l
     // need per utterance
     const long long more = n_utt < M ? n_utt : M, mean = M / more;
     pick_tile(N, more * ((mean + 127) / 128), more * ((mean + 255) / 256), K, &bn, &pair);
-    int rc = common(c, bn, pair, p, m);
+    int rc = common(c, false, bn, pair, p, m);
     if (rc) return rc;
     p.off = off;
     p.T = T;

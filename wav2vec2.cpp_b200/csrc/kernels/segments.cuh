@@ -72,7 +72,8 @@ __host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, i
 
 // Fills the plan: lora_shrink.cu.  The launch lets the next kernel of the
 // stream start early; that one waits (grid_dependency_wait) before it reads the plan.
-int lora_shrink(const LoraArgs& a, const LoraPlan& p, cudaStream_t st);
+// x: a map of the rows in boxes of x_rows, if the caller has one.
+int lora_shrink(const LoraArgs& a, const LoraPlan& p, const CUtensorMap* x, int x_rows, cudaStream_t st);
 
 inline PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
