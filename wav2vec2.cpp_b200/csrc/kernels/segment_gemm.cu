@@ -119,9 +119,10 @@ struct Walker {
         total = 0;
         return n;
     }
-    // m < count(), not below an earlier call's
-    W2V_DEV void find(const Params& p, int tile_rows, int m, Tile& t) {
+    // m not below an earlier call's; false: there are no more
+    W2V_DEV bool find(const Params& p, int tile_rows, int m, Tile& t) {
         while (m >= before + total) {
+            if (base + 32 >= p.n_utt) return false;
             before += total;
             base += 32;
             load(p, tile_rows);
@@ -133,6 +134,7 @@ struct Walker {
         t.row0 = uniform(__shfl_sync(0xffffffffu, first, src) + k * tile_rows);
         t.end = uniform(__shfl_sync(0xffffffffu, end, src));
         t.group = uniform(__shfl_sync(0xffffffffu, group, src));
+        return true;
     }
 };
 
@@ -296,7 +298,17 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
     const int n_units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
-    if (threadIdx.x == 0) {
+    Walker walk;
+    auto tile_at = [&](int tile, Tile& t) {
+        t.ni = tile % p.n_tiles;
+        const int m = tile / p.n_tiles;
+        if constexpr (LORA) { t.row0 = m * kTileRows; t.end = p.M; t.group = 0; return true; }
+        else return walk.find(p, kTileRows, m, t);
+    };
+    Tile tile0 = {};                           // the producer's first, found while the others set up
+    bool any = true;
+    if (!LORA && warp == 0) any = tile_at(unit, tile0);
+    if (threadIdx.x == 32 * (kThreads / 32 - 1)) {
         for (int s = 0; s < S; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], kNE * CT); }
         mbar_init(done, 1);
@@ -319,16 +331,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     auto accumulator_at = [&](uint32_t i) {
         return tmem_base + (n_sums > 1 ? (uint32_t)p.bn * (1u + i) : i * 256u);
     };
-    Walker walk;
-    const int total = (LORA ? p.m_tiles : walk.count(p, kTileRows)) * p.n_tiles;
-    auto tile_at = [&](int tile) {
-        Tile t;
-        t.ni = tile % p.n_tiles;
-        const int m = tile / p.n_tiles;
-        if constexpr (LORA) { t.row0 = m * kTileRows; t.end = p.M; t.group = 0; }
-        else walk.find(p, kTileRows, m, t);
-        return t;
-    };
+    // the producer walks until there are no more tiles; the others count them while it loads the first
+    const int total = (LORA || warp == 0 ? p.m_tiles : walk.count(p, kTileRows)) * p.n_tiles;
     // further K-blocks of a row tile: adapters x parts x steps of 64 ranks
     const int chunks = LORA ? (p.plan.rank + kBK - 1) / kBK : 0;
 
@@ -362,8 +366,9 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             last_par = (last_par & ~(1u << stage)) | (phase << stage);
             if (++stage == S) { stage = 0; phase ^= 1u; }
         };
-        for (int tile = unit; tile < total && ok; tile += n_units) {
-            const Tile t = tile_at(tile);
+        for (int tile = unit; tile < total && any && ok; tile += n_units) {
+            Tile t = tile0;
+            if ((LORA || tile != unit) && !tile_at(tile, t)) break;
             const int col0 = t.ni * p.bn;
             if constexpr (LORA) {
                 arm_bytes = (uint32_t)(CT * (p.b_bytes + p.a_rows * kBK * 2));
@@ -469,7 +474,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         constexpr bool kF16 = EPI == W2V_EPI_F16 || EPI == W2V_EPI_F16_GELU;
         uint32_t nst = 0, acc = 0, acc_phase = 0;
         for (int tile = unit; tile < total; tile += n_units) {
-            const Tile t = tile_at(tile);
+            Tile t;
+            tile_at(tile, t);
             const int row0 = t.row0 + (int)rank * kBM + q * 32;
             const int col0 = t.ni * p.bn;
             const float* bias = p.bias ? p.bias + (long long)t.group * p.bias_stride : nullptr;
