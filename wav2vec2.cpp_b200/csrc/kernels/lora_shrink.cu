@@ -6,14 +6,25 @@
 // the read of x bounds it, and the time from a block's start to its end where
 // there are few rows.  A block takes 128 rows, or 64 where those are few or the
 // row tile is no multiple of 128 (the MMA's other 64 rows are then whatever lies
-// behind them).  A ring of stages holds 64 columns of x and of A_a; a warp of its
-// own fills it by TMA, x at once and A_a when the other four have looked the
-// block's adapters up.  tcgen05.mma multiplies a stage by each of two adapters, if
-// the rows use two, into accumulators side by side in TMEM, so that a block that
-// sees the end of an utterance takes hardly longer than the others.  (With
-// m16n8k16 MMAs in registers their rate was the bound: 60 x 10 s, K 1024, rank 64
-// took 31 us.)  More adapters (single frames) are taken in turn, by other
-// blocks where there are few rows.
+// behind them).  Nine warps: four look up the block's adapters (the plan) and write
+// the results, one fills a ring of stages of 64 columns of x and of A_a by TMA, x
+// at once and A_a when the plan is there, and up to four multiply.  A stage meets
+// each of two adapters, if the rows use two, in accumulators side by side in TMEM,
+// so that a block that sees the end of an utterance takes hardly longer than the
+// others; more are taken in turn, by other blocks where there are few rows.
+// (With m16n8k16 MMAs in registers their rate was the bound: 60 x 10 s, K 1024,
+// rank 64 took 31 us.)
+//
+// Four issuing warps: a stage's wait, MMAs and commit cost one warp some 500 cycles
+// where the tensor core takes 184 (four MMAs of 16 columns), a stage after the other.
+// Each takes every fourth stage into accumulators of its own, which are added when
+// they are read.
+//
+// Few rows (kDirect): what counts is the way from the launch to the results.
+// Each adapter has a block of its own whether the rows use it or not, which loads and
+// multiplies before the plan is there.  Projections with adapters, the whole call
+// (one warp and the plan first -> these two): 16 single frames of 8 adapters, K = N = 1024,
+// 15.0 -> 13.1 us; 499 rows, K = N = 768, 4 adapters 12.3 -> 10.6 us.
 #include "segments.cuh"
 #include "w2v_kernels.h"
 
@@ -23,6 +34,8 @@ namespace sg {
 constexpr int kStep = 64, kMaxTile = 256;
 constexpr int kPlanners = 128, kProducer = kPlanners / 32, kIssuers = 4, kThreads = kPlanners + 32 + 32 * kIssuers;
 constexpr int kMaxRing = 8;
+// Blocks up to which each adapter has its own: up to 32 the call gains 0.6 to 1.8 us (of 10 to 24);
+// at 64 some gain 0.2 to 1.0, others lose 1.9 to 2.5, the blocks standing where the projection's would start.
 constexpr int kDirect = 32;
 
 struct ShrinkShape {
