@@ -41,6 +41,8 @@
 // extra on the barriers of eight search warps.
 #include <float.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "w2v_kernels.h"
 
@@ -102,6 +104,7 @@ struct Params {
     int* err;
     int n_pairs;         // extension candidates (i, j): (i + 1) j <= width
     int slots;           // rows in the ring
+    int copied;          // nodes that fit there for the hypotheses
 };
 
 // Tokens of rank 0 .. n_tok - 1 can extend a beam.
@@ -157,7 +160,7 @@ __host__ __device__ constexpr int max_live(int MW) {
 }
 
 template <int MW>
-struct Shared {
+struct alignas(16) Shared {          // (what lies behind it is read 16 bytes at a time)
     uint32_t key32[max_live(MW)];    // leading bits of the values of the candidates in the running
     u64 key[max_live(MW)];           // the values
     Beams<MW> beams[2];
@@ -172,6 +175,7 @@ struct Shared {
     uint32_t least_hi[8];
     // of the last frame, for the hypotheses
     int nb, cur;
+    int n_nodes;
     long long exp2, z_exp2;
     double z;
 };
@@ -746,6 +750,7 @@ __global__ void __launch_bounds__((NC + NP + 1) * 32, 1) ctc_beam_kernel(Params 
             s.nb = refused || failed ? 0 : nb;
             s.cur = cur;
             s.exp2 = exp2;
+            s.n_nodes = refused || failed ? 0 : 1 + (frames + T) * W;
             if (failed) hdr->tag = 0;
         }
         // state for the next call
@@ -766,23 +771,52 @@ __global__ void __launch_bounds__((NC + NP + 1) * 32, 1) ctc_beam_kernel(Params 
     if (p.n_best == 0) return;
     __syncthreads();
     // hypotheses, best first
+    constexpr int kWarps = NC + NP + 1;
     const Beams<MW>& b = s.beams[s.cur];
     const int have = s.nb < p.n_best ? s.nb : p.n_best;
-    for (int h = warp; h < p.n_best; h += NC + NP + 1) {
+    for (int h = warp; h < p.n_best; h += kWarps) {
+        const int len = h < have ? b.info[h].len : 0;
+        int* out = p.ids + ((long long)u * p.n_best + h) * p.cap;
+        for (long long i = len + lane; i < p.cap; i += 32) out[i] = -1;
+    }
+    // A lane each walks from its hypothesis' node up, through a copy of the nodes in shared memory, newest
+    // first (a node's parent is older): a step from global memory takes some 300 ns, and a stream's call of few
+    // frames would spend more on the walk than on the frames.
+    static_assert(kWarps * 32 >= MW, "a lane for each hypothesis");
+    const int h = lane * kWarps + warp;
+    int id = -1, left = 0;               // left: tokens still to be found
+    int* out = nullptr;
+    if (h < p.n_best) {
         const long long at = (long long)u * p.n_best + h;
         const int len = h < have ? b.info[h].len : -1;
-        int* out = p.ids + at * p.cap;
-        for (long long i = (len > 0 ? len : 0) + lane; i < p.cap; i += 32) out[i] = -1;
-        if (lane) continue;
         p.n_ids[at] = len;
         p.scores[at] = h < have ? log(b.prob[h].total) - log(s.z) + (double)(s.exp2 - s.z_exp2) * 0.69314718055994530942
-                               : -INFINITY;
-        if (len > 0)
-            for (int i = len - 1, id = b.info[h].node; i >= 0; i--) {
-                const Node nd = nodes[id];
-                if (i < p.cap) out[i] = nd.tok;
-                id = nd.parent;
-            }
+                                : -INFINITY;
+        if (len > 0) {
+            id = b.info[h].node;
+            left = len;
+            out = p.ids + at * p.cap;
+        }
+    }
+    int2* copy = reinterpret_cast<int2*>(rows);
+    for (int hi = s.n_nodes, lo; __syncthreads_or(left > 0) && hi > 0; hi = lo) {
+        lo = max(hi - p.copied, 0);
+        constexpr int kStep = kWarps * 32;
+        for (int k0 = lo + tid; k0 < hi; k0 += 8 * kStep) {
+            int2 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (k0 + e * kStep < hi) v[e] = *reinterpret_cast<const int2*>(nodes + k0 + e * kStep);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (k0 + e * kStep < hi) copy[k0 + e * kStep - lo] = v[e];
+        }
+        __syncthreads();
+        while (left > 0 && id >= lo && id < hi) {
+            const int2 v = copy[id - lo];            // parent, token
+            if (--left < p.cap) out[left] = v.y;
+            id = v.x;
+        }
     }
 }
 
@@ -791,7 +825,11 @@ static int launch(Params p, int n_utt, cudaStream_t st) {
     const long long fixed = (long long)sizeof(Shared<MW>) + (p.width * ((p.V + 31) / 32) * 4 + 15) / 16 * 16;
     const long long row = row_bytes(p.V, p.width);
     p.slots = fixed + 2 * NP * row <= 200 * 1024 ? 2 * NP : NP;
-    const long long smem = fixed + p.slots * row;
+    // room for the nodes too, no more than leaves as many blocks on an SM as there are
+    long long smem = fixed + p.slots * row;
+    const long long all = fixed + ((long long)p.width * p.max_frames + 1) * (long long)sizeof(int2);
+    if (p.n_best) smem = std::max(smem, std::min(all, 200 * 1024LL / ((n_utt + 147) / 148)));
+    p.copied = (int)((smem - fixed) / (long long)sizeof(int2));
     static bool attr[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
