@@ -36,8 +36,8 @@
 //
 // Bound: the chain of frames, each a row of dependent instructions, shuffles and
 // shared-memory round trips of few warps; a block holds an utterance, so 148 utterances
-// take as long as one.  32 tokens, width 16: 1.05 us a frame (499 frames 0.53 ms, 64
-// utterances of up to 499 0.55 ms); 94 tokens, width 100, 30 s: 2.1 us a frame, the
+// take as long as one.  32 tokens, width 16: 1.05 us a frame (499 frames 0.51 ms, 64
+// utterances of up to 499 0.53 ms); 94 tokens, width 100, 30 s: 2.0 us a frame, the
 // extra on the barriers of eight search warps.
 #include <float.h>
 
