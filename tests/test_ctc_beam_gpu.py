@@ -273,6 +273,20 @@ def test_state_that_was_not_started(K):
     assert b.results() == [[]] and int(b.err.item()) == 2
 
 
+@pytest.mark.parametrize("n_utt,T,V,width,n_best", [(1, 220, 4, 128, 100), (300, 600, 5, 16, 3)])
+def test_more_nodes_than_fit_beside_the_search(K, n_utt, T, V, width, n_best):
+    """Hypotheses whose nodes are read in several pieces; more utterances than SMs."""
+    lg = ctc_logits(np.random.default_rng(12), T, V, 0)
+    b = Beam(K, [lg] * n_utt, 0, width, n_best)
+    b.call()
+    got = b.results()
+    ref = search(lg, 0, width)[:n_best]
+    assert len(ref) == n_best and len(ref[0][0]) > T // 8
+    for hyps in got:
+        assert [g[0] for g in hyps] == [r[0] for r in ref]
+        assert all(abs(g[1] - r[1]) <= 1e-9 * (1 + abs(r[1])) for g, r in zip(hyps, ref))
+
+
 def test_short_id_rows(K):
     """n_ids has the whole length, ids the tokens that fit."""
     lg = np.full((12, 4), -9.0, np.float32)
