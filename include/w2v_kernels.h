@@ -223,8 +223,8 @@ int w2v_ctc_greedy(const float* logits, const long long* off, const int* T, int 
  * lora_b of an adapter in use must be finite: an infinity or NaN there may
  * reach the rows of other utterances nearby (at most 256 rows away).
  * A, W, lora_a, lora_b (and Bs) 16-byte aligned.  s_a lora_a[a] A[r] is held
- * in fp16 (as two numbers, value and remainder, for the fp32 epilogues): its
- * magnitude must stay below 65504. */
+ * as two fp16 numbers, value and remainder: to 2^-22 of it, and to no less than
+ * 2^-25; its magnitude must stay below 65504. */
 long long w2v_lora_workspace_bytes(long long M, int n_utt, int rank);
 int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long long M, const void* B, int N, void* C,
                       long long ldc, const float* bias, const float* resid, long long ldr, int epilogue,

@@ -95,7 +95,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* ring = smem_raw + (((raw + 1023u) & ~1023u) - raw);
     const int S = shape.stages;
-    const int rank = p.rank, n16 = (rank + 15) / 16 * 16, a_bytes = rank * kStep * 2;
+    const int rank = p.rank, n16 = rank16(rank), a_bytes = rank * kStep * 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long row0 = (long long)blockIdx.x * kRows;
     const long long tile = row0 / p.tile;
@@ -103,7 +103,6 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const int n_rows = (int)min((long long)p.tile, a.M - tile0);
     const int local0 = (int)(row0 - tile0);
     const int k_steps = a.K / kStep;
-    const long long part = p.blocks * p.tile * rank;
     const bool direct = shape.direct != 0;
     // the block that is sure to use its rows fetches the first of them before it knows the adapters
     const int early = blockIdx.y == 0 && !direct ? min(S, k_steps) : 0;
@@ -345,12 +344,9 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         }
         if (blockIdx.y == 0 && !direct)           // the others' blocks are zero in these rows
             for (int k = n_here; k < count; k++) {
-                __half* out = p.t + ((first_block + here[k]) * p.tile + local0) * rank;
-                const int n = min(kRows, n_rows - local0) * rank / 8;
-                for (int c = tid; c < n; c += kPlanners) {
-                    reinterpret_cast<uint4*>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
-                    if (p.parts == 2) reinterpret_cast<uint4*>(out + part)[c] = make_uint4(0u, 0u, 0u, 0u);
-                }
+                __half* out = p.t + ((first_block + here[k]) * p.tile + local0) * t_columns(rank);
+                const int n = min(kRows, n_rows - local0) * t_columns(rank) / 8;
+                for (int c = tid; c < n; c += kPlanners) reinterpret_cast<uint4*>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
             }
         if (tid == 0) n_here_shared = n_here;
     }
@@ -382,13 +378,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     } else {
         const uint32_t tmem = (uint32_t)uniform((int)tmem_slot);
         const int parts = min(issuers, k_steps);
-        // an adapter's share, masked, as fp16 (and what the rounding left, for fp32 outputs): a row per lane
+        // an adapter's share, masked, as fp16 and what the rounding left: a row per lane
         const int r = warp * 32 + lane;
         const bool real = local0 + r < n_rows;
         const int mine = row_slot[r];
         auto store = [&](int e, int s) {
             const float sc = a.scale ? a.scale[slots[s]] : 1.f;
-            __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * rank;
+            __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * t_columns(rank);
             for (int c = 0; c < rank; c += 16) {
                 const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * n16 + c);
                 float v[16];
@@ -402,21 +398,21 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                 uint32_t hi[8], low[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float v0 = mine == s ? v[2 * i] * sc : 0.f, v1 = mine == s ? v[2 * i + 1] * sc : 0.f;
+                    const bool has = mine == s && c + 2 * i < rank;      // (the columns behind the rank hold anything)
+                    const float v0 = has ? v[2 * i] * sc : 0.f, v1 = has ? v[2 * i + 1] * sc : 0.f;
                     const __half2 h = __floats2half2_rn(v0, v1);
                     const float2 f = __half22float2(h);
                     hi[i] = *reinterpret_cast<const uint32_t*>(&h);
                     low[i] = pack_half2(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
                 }
                 if (!real) continue;
-                uint4* o = reinterpret_cast<uint4*>(out + c);
-                uint4* o2 = reinterpret_cast<uint4*>(out + part + c);
+                const int r0 = c / kGroup * kGroup;
+                uint4* o = reinterpret_cast<uint4*>(out + 2 * r0 + (c - r0));
+                uint4* o2 = reinterpret_cast<uint4*>(out + 2 * r0 + group_width(rank, r0) + (c - r0));
                 o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (p.parts == 2) o2[0] = make_uint4(low[0], low[1], low[2], low[3]);
-                if (c + 16 <= rank) {
-                    o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                    if (p.parts == 2) o2[1] = make_uint4(low[4], low[5], low[6], low[7]);
-                }
+                o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                o2[0] = make_uint4(low[0], low[1], low[2], low[3]);
+                o2[1] = make_uint4(low[4], low[5], low[6], low[7]);
             }
         };
         if (direct) {

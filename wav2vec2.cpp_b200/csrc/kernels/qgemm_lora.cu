@@ -75,17 +75,17 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
     QLora<true> lo;
     lo.t = lo.b = m.x;
     lo.lora = n_utt > 0;
-    lo.plan = sg::lora_plan(workspace, M, n_utt, rank, rows, f16 ? 1 : 2);
+    lo.plan = sg::lora_plan(workspace, M, n_utt, rank, rows);
     // as the fp16 kernel does (segment_gemm.cu): 512 of K, 1024 beside a residual
     lo.sum_blocks = epilogue == W2V_EPI_F32_RESID ? 16 : 8;
     lo.n_sums = f16 ? 1 : (int)((K / kBK + lo.sum_blocks - 1) / lo.sum_blocks);
     lo.chunks = (2 * rank + code_row_bytes(wq) - 1) / code_row_bytes(wq);
     if (lo.lora) {
-        if (lo.plan.parts * lo.plan.blocks * rows > 0x7fffffffLL) return W2V_ERR_ARGS;
+        if (lo.plan.blocks * rows > 0x7fffffffLL) return W2V_ERR_ARGS;
         auto enc = get_encode();
         const uint32_t es[3] = {1, 1, 1};
-        const uint64_t td[2] = {(uint64_t)rank, (uint64_t)(lo.plan.parts * lo.plan.blocks * rows)};
-        const uint64_t ts[1] = {(uint64_t)rank * 2};
+        const uint64_t td[2] = {(uint64_t)sg::t_columns(rank), (uint64_t)(lo.plan.blocks * rows)};
+        const uint64_t ts[1] = {(uint64_t)sg::t_columns(rank) * 2};
         const uint32_t tbox[2] = {kBK, (uint32_t)(bn < 0 ? rows / 2 : rows)};
         if (enc(&lo.t, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, lo.plan.t, td, ts, tbox, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -39,7 +39,8 @@
 // activation rows (segments.cuh) is the B operand and the adapter's second
 // matrix, [N][rank] fp16, the A operand.  Its rows come through the code
 // boxes (same bytes per row: 32 ranks per k-block beside Q8_0 codes, 16 beside
-// Q4_0) and the converters copy them to tensor memory as they are.
+// Q4_0) and the converters copy them to tensor memory as they are; the value and the
+// remainder of the first product, both in the k-block's box, are multiplied by them in turn.
 #pragma once
 #include "segments.cuh"
 #include "w2v_kernels.h"
@@ -53,6 +54,9 @@ constexpr int kNC = 4;              // converter warps (epilogue warps: QCfg::kN
 constexpr int kSmemCap = 232448;
 enum : int { kQ8 = 1, kQ4 = 2 };
 __host__ __device__ constexpr int code_row_bytes(int wq) { return wq == kQ8 ? 64 : 32; }
+// Ranks of an adapter's k-block.
+template <int WQ>
+constexpr int kLoraRanks = code_row_bytes(WQ) / 2;
 __host__ __device__ constexpr int cmin(int a, int b) { return a < b ? a : b; }
 
 struct QParams {
@@ -76,10 +80,10 @@ template <bool LORA>
 struct QLora {};
 template <>
 struct QLora<true> {
-    CUtensorMap t;       // [parts][blocks][tile] rows of [rank] fp16, boxes of 64 x (rows one CTA stages)
+    CUtensorMap t;       // [blocks][tile] rows of t_columns(rank) fp16, boxes of 64 x (rows one CTA stages)
     CUtensorMap b;       // [n_adapters][N] rows of [rank] fp16 as bytes, boxes like the codes'
     sg::LoraPlan plan;
-    int chunks;          // k-blocks per adapter and part
+    int chunks;          // k-blocks per adapter
     int lora;            // the plan holds adapters
     int sum_blocks, n_sums;   // fp32 outputs: k-blocks of a sum, sums of a tile (segment_gemm.cu)
 };
@@ -263,18 +267,18 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                     if (!lo.lora) continue;
                     if (tile == unit) sg::grid_dependency_wait();
                     const sg::LoraTile lt = lo.plan.tiles[ri];
-                    for (int i = 0; i < lt.count * lo.plan.parts * lo.chunks && ok; i++) {
-                        const int c = i % lo.chunks, part = i / lo.chunks % lo.plan.parts;
-                        const int blk = lt.first + i / (lo.chunks * lo.plan.parts);
-                        const int trow = (int)((part * lo.plan.blocks + blk) * BN) + (int)rank * Cfg::kXRows;
+                    for (int i = 0; i < lt.count * lo.chunks && ok; i++) {
+                        const int c = i % lo.chunks, blk = lt.first + i / lo.chunks;
+                        const int trow = blk * BN + (int)rank * Cfg::kXRows;
+                        const int tcol = c * kLoraRanks<WQ> / sg::kGroup * 2 * sg::kGroup;   // of the ranks' group
                         if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) { ok = false; break; }
                         if constexpr (PAIR) {
                             if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::kXBytes);
                             tma_load_2d_pair(sX + stage * Cfg::kXBytes, &lo.t, full_lead + (uint32_t)(stage * 8),
-                                             c * code_row_bytes(WQ) / 2, trow);
+                                             tcol, trow);
                         } else {
                             mbar_arrive_expect_tx(&full[stage], Cfg::kXBytes);
-                            tma_load_2d(sX + stage * Cfg::kXBytes, &lo.t, &full[stage], c * code_row_bytes(WQ) / 2, trow);
+                            tma_load_2d(sX + stage * Cfg::kXBytes, &lo.t, &full[stage], tcol, trow);
                         }
                         mbar_arrive_expect_tx(&cfull[stage], Cfg::kCodeBytes);
                         tma_load_3d(sQ + stage * Cfg::kCodeBytes, &lo.b, &cfull[stage], c * code_row_bytes(WQ), frow,
@@ -334,15 +338,29 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                     tc_fence_after();
                     const uint32_t a0 = tmem_base + (uint32_t)(Cfg::kACol + f * 32);
                     const uint32_t b0 = smem_u32(sX + stage * Cfg::kXBytes);
-#pragma unroll
-                    for (int kk = 0; kk < kBK / 16; kk++) {
-                        if (LORA && kb >= p.k_blocks && kk >= code_row_bytes(WQ) / 32) break;
+                    // 16 columns of the weights from kw on by as many of the rows from kx on
+                    auto multiply = [&](int kw, int kx, bool add) {
                         if constexpr (PAIR)
-                            umma_f16_pair_tmem_a(d, a0 + (uint32_t)(kk * 8), umma_desc_sw128(b0 + kk * 32), idesc,
-                                                 kb != first_kb || kk != 0);
+                            umma_f16_pair_tmem_a(d, a0 + (uint32_t)(kw / 2), umma_desc_sw128(b0 + kx * 2), idesc, add);
                         else
-                            umma_f16_tmem_a(d, a0 + (uint32_t)(kk * 8), umma_desc_sw128(b0 + kk * 32), idesc,
-                                            kb != first_kb || kk != 0);
+                            umma_f16_tmem_a(d, a0 + (uint32_t)(kw / 2), umma_desc_sw128(b0 + kx * 2), idesc, add);
+                    };
+                    bool main = true;
+                    if constexpr (LORA)
+                        if (kb >= p.k_blocks) {              // ranks r0 + at .. of an adapter: value and remainder
+                            main = false;
+                            const int r = (kb - p.k_blocks) % lo.chunks * kLoraRanks<WQ>, r0 = r / sg::kGroup * sg::kGroup, at = r - r0;
+                            const int w = sg::group_width(lo.plan.rank, r0);
+#pragma unroll
+                            for (int k = 0; k < kLoraRanks<WQ>; k += 16)
+                                if (at + k < w) {
+                                    multiply(k, at + k, true);
+                                    multiply(k, w + at + k, true);
+                                }
+                        }
+                    if (main) {
+#pragma unroll
+                        for (int k = 0; k < kBK; k += 16) multiply(k, k, kb != first_kb || k != 0);
                     }
                     if constexpr (PAIR) {
                         umma_commit_pair(smem_u32(&empty[stage]));
@@ -357,7 +375,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                     if constexpr (LORA)
                         if (kb == p.k_blocks - 1 && lo.lora) {     // the main k-blocks are issued: the adapters'
                             if (tile == unit) sg::grid_dependency_wait();
-                            n_kb += lo.plan.tiles[tile / p.f_tiles].count * lo.plan.parts * lo.chunks;
+                            n_kb += lo.plan.tiles[tile / p.f_tiles].count * lo.chunks;
                         }
                 }
                 if (ok) {
@@ -389,7 +407,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                 if constexpr (LORA)
                     if (kb == p.k_blocks - 1 && lo.lora) {
                         if (tile == unit) sg::grid_dependency_wait();
-                        n_kb += lo.plan.tiles[tile / p.f_tiles].count * lo.plan.parts * lo.chunks;
+                        n_kb += lo.plan.tiles[tile / p.f_tiles].count * lo.chunks;
                     }
                 if (!mbar_wait(&cfull[s], (uint32_t)(kq / S) & 1u, p.err)) {
                     ok = false;

@@ -54,7 +54,9 @@ constexpr int kSmemCap = 232448;
 constexpr int kABytes = kBM * kBK * 2;
 constexpr int kEpiBytes = kNE * 4096;          // per warp: a 32 x 32 fp32 chunk, or two fp16 store boxes
 constexpr int kMaxStages = 8;
-constexpr uint32_t kLastOfTile = 16, kLastOfSum = 32;   // beside a stage's number of MMA steps
+// A stage's work: its number of MMA steps, these, and a mask from kWrap on: step k takes columns 16 k of
+// the rows and 16 (k & mask) of the weights (an adapter's value and remainder meet the same ones).
+constexpr uint32_t kLastOfTile = 16, kLastOfSum = 32, kWrap = 8, kMainWork = kBK / 16 | (kBK / 16 - 1) << kWrap;
 __host__ __device__ constexpr bool sums_of(int epi) { return epi == W2V_EPI_F32 || epi == W2V_EPI_F32_RESID; }
 // K-blocks of a sum: 512 of K; beside a residual, which as a rule is larger than what is added to it, 1024.
 __host__ __device__ constexpr int sum_blocks(int epi) { return epi == W2V_EPI_F32_RESID ? 16 : 8; }
@@ -339,8 +341,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     };
     // the producer walks until there are no more tiles; the others count them while it loads the first
     const int total = (LORA || warp == 0 ? p.m_tiles : walk.count(p, kTileRows)) * p.n_tiles;
-    // further K-blocks of a row tile: adapters x parts x steps of 64 ranks
-    const int chunks = LORA ? (p.plan.rank + kBK - 1) / kBK : 0;
+    // further K-blocks of a row tile: adapters x groups of 32 ranks
+    const int chunks = LORA ? (p.plan.rank + kGroup - 1) / kGroup : 0;
 
     if (warp == 0) {
         // the leader's barriers count the bytes of a pair
@@ -355,7 +357,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // grouped: of the rows only the 32-row boxes that hold valid ones, where that saves any (tmT, which is
         // theirs then): what the MMA reads in the others' places goes to accumulator rows that are not stored
         int boxes = 4;
-        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int k, int ra, int rb, int gb, uint32_t work) {
+        // k, kw: first column of the rows' and of the weights' tile
+        auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int k, int ra, int rb, int gb, uint32_t work, int kw) {
             if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
             const uint32_t dst = base + (uint32_t)(stage * stage_bytes), bar = full_lead + (uint32_t)(stage * 8);
             if (WORK && lane == 0) stage_work[stage] = work;
@@ -367,7 +370,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 for (int i = 0; i < boxes; i++)
                     tma_load_2d_if<PAIR>(lead, dst + (uint32_t)(i * kABytes / 4), &tmT, bar, k, ra + (int)rank * kBM + i * 32);
             }
-            tma_load_3d_if<PAIR>(lead, dst + kABytes, mb, bar, k, rb + b_row, gb);
+            tma_load_3d_if<PAIR>(lead, dst + kABytes, mb, bar, kw, rb + b_row, gb);
             issued |= 1u << stage;
             last_par = (last_par & ~(1u << stage)) | (phase << stage);
             if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -385,7 +388,7 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             }
             for (int kb = 0; kb < p.k_blocks - 1 && ok; kb++)
                 stage_in(&tmA, &tmB, kb * kBK, t.row0, col0, t.group,
-                         kBK / 16 | (SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1 ? kLastOfSum : 0));
+                         kMainWork | (SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1 ? kLastOfSum : 0), kb * kBK);
             int blocks = 0, first = 0, rec = 0;
             if (LORA && p.lora) {
                 if (tile == unit) grid_dependency_wait();
@@ -395,17 +398,15 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 blocks = uniform(__shfl_sync(0xffffffffu, rec, 1));
             }
             if (ok)
-                stage_in(&tmA, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kBK / 16 | (blocks ? 0 : kLastOfTile | kLastOfSum));
+                stage_in(&tmA, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kMainWork | (blocks ? 0 : kLastOfTile | kLastOfSum), (p.k_blocks - 1) * kBK);
             for (int b = 0; b < blocks && ok; b++) {
                 const int held = __shfl_sync(0xffffffffu, rec, min(2 + b, 31));
                 const int ad = uniform(b < kInline ? held : p.plan.adapter[first + b]);
-                for (int part = 0; part < p.plan.parts; part++) {
-                    const int trow = (int)((part * p.plan.blocks + first + b) * kTileRows);
-                    for (int c = 0; c < chunks && ok; c++) {
-                        const bool last = b + 1 == blocks && part + 1 == p.plan.parts && c + 1 == chunks;
-                        stage_in(&tmT, &tmL, c * kBK, trow, col0, ad,
-                                 min(kBK / 16, (p.plan.rank - c * kBK + 15) / 16) | (last ? kLastOfTile | kLastOfSum : 0));
-                    }
+                for (int c = 0; c < chunks && ok; c++) {
+                    const uint32_t steps = (uint32_t)group_width(p.plan.rank, c * kGroup) / 16;
+                    const bool last = b + 1 == blocks && c + 1 == chunks;
+                    stage_in(&tmT, &tmL, c * kBK, (first + b) * kTileRows, col0, ad,
+                             2 * steps | (steps - 1) << kWrap | (last ? kLastOfTile | kLastOfSum : 0), c * kGroup);
                 }
             }
         }
@@ -436,9 +437,9 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tc_fence_after();
                     return true;
                 };
-                auto multiply = [&](uint32_t go, int kk) {
+                auto multiply = [&](uint32_t go, int kk, int kw) {
                     const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
-                    umma_f16_if<PAIR>(go, d, desc_plus(da, kk * 32), desc_plus(db, kk * 32), idesc, !first || kk != 0);
+                    umma_f16_if<PAIR>(go, d, desc_plus(da, kk * 32), desc_plus(db, kw * 32), idesc, !first || kk != 0);
                 };
                 auto end = [&](bool last_of_sum) {
                     umma_commit_if<PAIR>(lead, empty_here + (uint32_t)(stage * 8));
@@ -456,15 +457,16 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 for (int kb = 0; kb < p.k_blocks - 1; kb++) {
                     if (!begin()) { ok = false; break; }
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; kk++) multiply(lead, kk);
+                    for (int kk = 0; kk < kBK / 16; kk++) multiply(lead, kk, kk);
                     end(SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1);
                 }
                 // the last of K and the adapters' stages: as the producer found them
                 for (uint32_t work = 0; ok && !(work & kLastOfTile);) {
                     if (!begin()) { ok = false; break; }
-                    work = WORK ? (uint32_t)uniform((int)stage_work[stage]) : kBK / 16 | kLastOfSum | kLastOfTile;
+                    work = WORK ? (uint32_t)uniform((int)stage_work[stage]) : kMainWork | kLastOfSum | kLastOfTile;
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; kk++) multiply(LORA ? lead & (uint32_t)(kk < (int)(work & 15u)) : lead, kk);
+                    for (int kk = 0; kk < kBK / 16; kk++)
+                        multiply(LORA ? lead & (uint32_t)(kk < (int)(work & 15u)) : lead, kk, LORA ? kk & (int)(work >> kWrap) : kk);
                     end((work & kLastOfSum) != 0);
                 }
             }
@@ -755,11 +757,11 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
     const int tile_rows = pair ? 256 : 128;
     p.m_tiles = (int)((M + tile_rows - 1) / tile_rows);
     p.lora = n_utt > 0;
-    p.plan = lora_plan(workspace, M, n_utt, rank, tile_rows, epilogue == W2V_EPI_F16 || epilogue == W2V_EPI_F16_GELU ? 1 : 2);
+    p.plan = lora_plan(workspace, M, n_utt, rank, tile_rows);
     if (p.lora) {
-        if (p.plan.parts * p.plan.blocks * tile_rows > 0x7fffffffLL) return W2V_ERR_ARGS;
-        const uint64_t td[2] = {(uint64_t)rank, (uint64_t)(p.plan.parts * p.plan.blocks * tile_rows)};
-        const uint64_t ts[1] = {(uint64_t)rank * 2};
+        if (p.plan.blocks * tile_rows > 0x7fffffffLL) return W2V_ERR_ARGS;
+        const uint64_t td[2] = {(uint64_t)t_columns(rank), (uint64_t)(p.plan.blocks * tile_rows)};
+        const uint64_t ts[1] = {(uint64_t)t_columns(rank) * 2};
         rc = map_f16(&m.t, p.plan.t, 2, td, ts, p.a_rows);
         if (rc) return rc;
         const uint64_t ld[3] = {(uint64_t)rank, (uint64_t)N, (uint64_t)n_adapters};

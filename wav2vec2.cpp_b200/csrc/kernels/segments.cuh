@@ -7,11 +7,18 @@
 namespace w2v {
 namespace sg {
 
-// Low-rank adapters: s_a A_a x of every row, laid out for a GEMM whose tiles
+// Low-rank adapters: t = s_a A_a x of every row, laid out for a GEMM whose tiles
 // take `tile` rows.  For each adapter that a tile's rows use there is a block
-// [tile][rank] of fp16, zero in the rows of other adapters, so that the
+// of `tile` rows of fp16, zero in the rows of other adapters, so that the
 // second product is (block) x (that adapter's B): further K-blocks of the
 // tile's main product, however the tile's rows are spread over utterances.
+//
+// t is held as two fp16 numbers, the value and what its rounding left: 22 bits, as
+// much as fp32 outputs need, and more than fp16 outputs can do without (with 11 bits
+// they are off by half a step of their own in one place of three).  They stand side by side,
+// 32 ranks of the one, then of the other, so that both meet the same columns of B within
+// one K-block: a row is groups of 64 columns, the last of 2 w where w = 16 or 32 ranks
+// are left (the rank rounded up to 16; zero behind it).
 // Tile i's blocks are first .. first + count - 1 with
 //   first = i + min(utterances that end before the tile, rows before it),
 // which leaves room for every tile without a scan over the tiles before: of a
@@ -24,10 +31,9 @@ struct LoraTile {          // 64 bytes: one load of half a warp
 struct LoraPlan {
     LoraTile* tiles;       // [row tiles]
     int* adapter;          // [blocks]
-    __half* t;             // [parts][blocks][tile][rank]
+    __half* t;             // [blocks][tile][t_columns(rank)]
     int tile;              // rows per tile: 64, 128, 192 or 256
     int rank;
-    int parts;             // 1: fp16; 2: value and remainder (fp32 outputs)
     long long blocks;      // room for so many
 };
 
@@ -46,6 +52,12 @@ struct LoraArgs {
     int* err;
 };
 
+constexpr int kGroup = 32;                                                     // ranks whose values stand together
+__host__ __device__ inline int rank16(int rank) { return (rank + 15) / 16 * 16; }
+__host__ __device__ inline int t_columns(int rank) { return 2 * rank16(rank); }
+// Ranks (rounded up to 16) of the group that begins at rank r.
+__host__ __device__ inline int group_width(int rank, int r) { return rank16(rank) - r < kGroup ? rank16(rank) - r : kGroup; }
+
 __host__ inline long long lora_blocks(long long M, int n_utt, int tile) {
     return (M + tile - 1) / tile + (n_utt < M ? n_utt : M);
 }
@@ -53,14 +65,13 @@ __host__ inline long long lora_blocks(long long M, int n_utt, int tile) {
 __host__ inline long long lora_workspace(long long M, int n_utt, int rank) {
     const long long rows = M + 256 * (1 + (n_utt < M ? n_utt : M));
     const long long tiles = M / 64 + 1;
-    return (tiles * (long long)sizeof(LoraTile) + 255) / 256 * 256 + ((tiles + (n_utt < M ? n_utt : M)) * 4 + 255) / 256 * 256 + rows * rank * 4 + 256;
+    return (tiles * (long long)sizeof(LoraTile) + 255) / 256 * 256 + ((tiles + (n_utt < M ? n_utt : M)) * 4 + 255) / 256 * 256 + rows * t_columns(rank) * 2 + 256;
 }
-__host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, int tile, int parts) {
+__host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, int tile) {
     LoraPlan p;
     uint8_t* at = reinterpret_cast<uint8_t*>(ws);
     p.tile = tile;
     p.rank = rank;
-    p.parts = parts;
     p.blocks = lora_blocks(M, n_utt, tile);
     p.tiles = reinterpret_cast<LoraTile*>(at);
     at += ((M + tile - 1) / tile * (long long)sizeof(LoraTile) + 255) / 256 * 256;
