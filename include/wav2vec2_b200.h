@@ -78,7 +78,11 @@ int wav2vec2_b200_device_outputs(struct wav2vec2_context * ctx, const float ** l
  * (tokens of a hypothesis, -1 where there are fewer; its natural-log
  * probability), ids [n_utt][n_best][cap] (the first cap tokens, -1 behind
  * them).  Enqueues on `stream`, which must follow the forward's (NULL: the
- * context's own stream, as there), and returns without synchronising. */
+ * context's own stream, as there), and returns without synchronising.
+ * Without such a batch (no forward_device yet, or one that failed) there is
+ * nothing to search and nothing is written.  After any other forward on the
+ * context's first device (a host batch, debug_stages), whose buffers these
+ * are, it is refused (W2V_STATUS_INVALID) until the next forward_device. */
 int wav2vec2_b200_beam_device(struct wav2vec2_context * ctx, int beam_width, int n_best, int * ids, long long cap,
                               int * n_ids, double * scores, void * stream);
 

@@ -443,7 +443,7 @@ int wav2vec2_b200_forward_device(wav2vec2_context* ctx, const float* d_audio, co
         Engine* e = ctx->engines[0].get();
         std::vector<int> ns(n_samples, n_samples + n_utt);
         BatchGeom g = e->geometry(ns);
-        e->forward(d_audio, g, reinterpret_cast<cudaStream_t>(stream));
+        e->forward_device(d_audio, g, reinterpret_cast<cudaStream_t>(stream));
     } catch (const std::exception& ex) {
         set_error(ex.what());
         return W2V_STATUS_CUDA;
@@ -514,8 +514,9 @@ int wav2vec2_b200_beam_device(wav2vec2_context* ctx, int beam_width, int n_best,
         return W2V_STATUS_INVALID;
     }
     try {
-        if (!ctx->engines[0]->beam(beam_width, n_best, ids, cap, n_ids, scores, reinterpret_cast<cudaStream_t>(stream))) {
-            set_error("invalid arguments");
+        Engine* e = ctx->engines[0].get();
+        if (!e->beam(beam_width, n_best, ids, cap, n_ids, scores, reinterpret_cast<cudaStream_t>(stream))) {
+            set_error(e->held_lost() ? "another forward has replaced the last device batch's logits" : "invalid arguments");
             return W2V_STATUS_INVALID;
         }
     } catch (const std::exception& ex) {

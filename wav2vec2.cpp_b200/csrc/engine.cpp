@@ -514,12 +514,12 @@ void Engine::upload_meta(const BatchGeom& g, cudaStream_t st) {
 bool Engine::beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st) {
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     if (!st) st = stream_;
-    const int frames = std::max(last_T_max_, 1);
-    const long long bytes = w2v_ctc_beam_state_bytes(last_n_utt_, cfg_.vocab, width, frames);
-    if (bytes < 0 || n_best < 1 || n_best > width || !ids || !n_ids || !scores || cap < 1) return false;
-    if (last_n_utt_ == 0) return true;
+    const int frames = std::max(held_T_max_, 1);
+    const long long bytes = w2v_ctc_beam_state_bytes(held_n_utt_, cfg_.vocab, width, frames);
+    if (bytes < 0 || n_best < 1 || n_best > width || !ids || !n_ids || !scores || cap < 1 || held_lost_) return false;
+    if (held_n_utt_ == 0) return true;
     beam_state_.ensure((size_t)bytes);
-    const int rc = w2v_ctc_beam(logits_.as<float>(), d_T_off_, d_T_, last_n_utt_, cfg_.vocab, cfg_.pad_id, width, frames, 0,
+    const int rc = w2v_ctc_beam(logits_.as<float>(), d_T_off_, d_T_, held_n_utt_, cfg_.vocab, cfg_.pad_id, width, frames, 0,
                                 beam_state_.p, bytes, n_best, ids, cap, n_ids, scores, err_.as<int>(), st);
     if (rc == W2V_ERR_ARGS) return false;
     if (rc != W2V_OK) throw std::runtime_error("ctc_beam: status " + std::to_string(rc));
@@ -544,13 +544,12 @@ int Engine::check_device_error() {
 bool Engine::fwd_begin(const BatchGeom& g, cudaStream_t st) {
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     last_M_ = g.M;
-    last_n_utt_ = 0;                 // until the buffers hold this batch
-    last_T_max_ = g.T_max;
+    held_lost_ = held_lost_ || held_n_utt_ > 0;
+    held_n_utt_ = 0;
     launches_cur_ = 0;
     if (g.n_utt == 0) { launches_last_ = 0; return false; }
     ensure_workspace(g);
     upload_meta(g, st);
-    last_n_utt_ = g.n_utt;
     if (g.M == 0) {
         cuda_check(cudaMemsetAsync(nspans_.p, 0, sizeof(int) * g.n_utt, st), "memset");
         launches_last_ = 0;
@@ -744,6 +743,14 @@ void Engine::forward(const float* d_audio, const BatchGeom& g, cudaStream_t st, 
     if (!st) st = stream_;
     if (!fwd_begin(g, st)) return;   // workspace and metadata upload: never part of a captured graph
     extract_encode(d_audio, g, st, dbg_feat, dbg_stages);
+}
+
+void Engine::forward_device(const float* d_audio, const BatchGeom& g, cudaStream_t st) {
+    held_n_utt_ = 0;
+    held_lost_ = false;
+    forward(d_audio, g, st);
+    held_n_utt_ = g.n_utt;           // (not after a forward that failed)
+    held_T_max_ = g.T_max;
 }
 
 void Engine::extract_encode(const float* d_audio, const BatchGeom& g, cudaStream_t st, float* dbg_feat,

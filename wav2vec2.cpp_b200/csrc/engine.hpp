@@ -108,9 +108,13 @@ public:
     const int* d_n_spans() const { return nspans_.as<int>(); }
     long long last_M() const { return last_M_; }
 
-    // Prefix beam search on the logits of the last forward (outputs on the
-    // device, as w2v_ctc_beam's); false: sizes that it does not take.
+    // forward() for a caller that keeps the outputs on the device: the batch that beam() searches.
+    void forward_device(const float* d_audio, const BatchGeom& g, cudaStream_t st);
+    // Prefix beam search on the logits of the last forward_device (outputs on
+    // the device, as w2v_ctc_beam's); false: sizes that it does not take, or
+    // another forward has taken the buffers since.
     bool beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st);
+    bool held_lost() const { return held_lost_; }
 
     // Device error word set by kernels whose bounded waits expired.
     int check_device_error();
@@ -183,7 +187,10 @@ private:
     DevBuf logits_, ids_, spans_, nspans_;
     DevBuf err_;
     long long last_M_ = 0;
-    int last_n_utt_ = 0, last_T_max_ = 0;
+    // The batch of forward_device whose logits the buffers hold, for beam(): none, or lost to another
+    // forward, whose utterances the caller of beam() has no room for.
+    int held_n_utt_ = 0, held_T_max_ = 0;
+    bool held_lost_ = false;
     DevBuf beam_state_;
     long long launches_cur_ = 0, launches_last_ = 0;
 
