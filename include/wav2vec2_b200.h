@@ -79,6 +79,8 @@ int wav2vec2_b200_device_outputs(struct wav2vec2_context * ctx, const float ** l
  * probability), ids [n_utt][n_best][cap] (the first cap tokens, -1 behind
  * them).  Enqueues on `stream`, which must follow the forward's (NULL: the
  * context's own stream, as there), and returns without synchronising.
+ * Searches, and the context's next forward, wait for the last search
+ * whatever their streams.
  * Without such a batch (no forward_device yet, or one that failed) there is
  * nothing to search and nothing is written.  After any other forward on the
  * context's first device (a host batch, debug_stages), whose buffers these

@@ -78,3 +78,60 @@ def test_host_batches_alone_leave_nothing_to_search(B, model_path, synth):
     torch.cuda.synchronize()
     assert o.untouched()
     m.close()
+
+
+def test_searches_and_forwards_on_several_streams(B, model_path, synth):
+    """Searches of one batch on three streams at once share the context's state buffer, and the
+    next forward, on a fourth, its logits: each gives what it gives alone."""
+    m = B.Model(model_path("tiny", "q8_0", bias_std=0.02, gain_jitter=0.1))
+    batches = []
+    for k in range(2):
+        xs = [synth.make_audio(30000 - 900 * i, 70 + 13 * k + i) for i in range(6 - 3 * k)]
+        batches.append((torch.from_numpy(np.concatenate(xs)).cuda(), [len(x) for x in xs]))
+    kinds = [(100, 5), (6, 3), (33, 2)]                       # (width, n best)
+    refs = []
+    for d, lens in batches:
+        refs.append([])
+        for width, best in kinds:
+            m.forward_device(d.data_ptr(), lens)
+            o = Outputs(len(lens), best, 120)
+            torch.cuda.synchronize()
+            o.search(m, width)
+            refs[-1].append(o.host())
+    streams = [torch.cuda.Stream() for _ in kinds]
+    forward = torch.cuda.Stream()
+    outs = [[[Outputs(len(b[1]), best, 120) for _, best in kinds] for b in batches] for _ in range(5)]
+    torch.cuda.synchronize()
+    for turn in outs:
+        for (d, lens), os in zip(batches, turn):
+            m.forward_device(d.data_ptr(), lens, forward.cuda_stream)
+            done = forward.record_event()
+            for s, o, (width, _) in zip(streams, os, kinds):
+                s.wait_event(done)
+                o.search(m, width, s.cuda_stream)
+    torch.cuda.synchronize()
+    for turn in outs:
+        for os, rs in zip(turn, refs):
+            for o, r in zip(os, rs):
+                assert same(o.host(), r) and o.untouched(o.n)
+    m.close()
+
+
+def test_captured_search(B, model_path, synth):
+    """A search captured into a graph after one like it has run, replayed after another."""
+    m = B.Model(model_path("tiny", "q8_0", bias_std=0.02, gain_jitter=0.1))
+    x = synth.make_audio(20000, 5)
+    d = torch.from_numpy(x).cuda()
+    torch.cuda.synchronize()
+    m.forward_device(d.data_ptr(), [len(x)])
+    a, b = Outputs(1, 2, 80), Outputs(1, 2, 80)
+    torch.cuda.synchronize()
+    a.search(m, 8)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b.search(m, 8, torch.cuda.current_stream().cuda_stream)
+    g.replay()
+    g.replay()
+    assert same(a.host(), b.host())
+    m.close()

@@ -184,6 +184,7 @@ Engine::Engine(const GgufFile& gf, const ModelConfig& cfg, int device) : cfg_(cf
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     cuda_check(cudaStreamCreateWithFlags(&stream_, cudaStreamNonBlocking), "cudaStreamCreate");
     cuda_check(cudaEventCreateWithFlags(&meta_done_, cudaEventDisableTiming), "cudaEventCreate");
+    cuda_check(cudaEventCreateWithFlags(&beam_done_, cudaEventDisableTiming), "cudaEventCreate");
     cuda_check(cudaStreamCreateWithFlags(&copy_stream_, cudaStreamNonBlocking), "cudaStreamCreate");
     for (auto& e : chunk_ev_) cuda_check(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "cudaEventCreate");
     cuda_check(cudaEventCreate(&busy0_), "cudaEventCreate");
@@ -223,6 +224,7 @@ Engine::~Engine() {
     prof_fold();
     for (auto e : ev_pool_) cudaEventDestroy(e);
     if (meta_done_) cudaEventDestroy(meta_done_);
+    if (beam_done_) cudaEventDestroy(beam_done_);
     if (busy0_) cudaEventDestroy(busy0_);
     if (busy1_) cudaEventDestroy(busy1_);
     for (auto e : chunk_ev_)
@@ -511,6 +513,12 @@ void Engine::upload_meta(const BatchGeom& g, cudaStream_t st) {
     cuda_check(cudaEventRecord(meta_done_, st), "meta event");
 }
 
+static bool capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    cuda_check(cudaStreamIsCapturing(st, &s), "capture status");
+    return s != cudaStreamCaptureStatusNone;
+}
+
 bool Engine::beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st) {
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     if (!st) st = stream_;
@@ -519,11 +527,21 @@ bool Engine::beam(int width, int n_best, int* ids, long long cap, int* n_ids, do
     if (bytes < 0 || n_best < 1 || n_best > width || !ids || !n_ids || !scores || cap < 1 || held_lost_) return false;
     if (held_n_utt_ == 0) return true;
     beam_state_.ensure((size_t)bytes);
+    wait_for_beam(st);
     const int rc = w2v_ctc_beam(logits_.as<float>(), d_T_off_, d_T_, held_n_utt_, cfg_.vocab, cfg_.pad_id, width, frames, 0,
                                 beam_state_.p, bytes, n_best, ids, cap, n_ids, scores, err_.as<int>(), st);
     if (rc == W2V_ERR_ARGS) return false;
     if (rc != W2V_OK) throw std::runtime_error("ctc_beam: status " + std::to_string(rc));
+    if (!capturing(st)) {
+        cuda_check(cudaEventRecord(beam_done_, st), "beam event");
+        beam_pending_ = true;
+    }
     return true;
+}
+
+// (A search in a stream that is being captured is ordered by whoever replays it.)
+void Engine::wait_for_beam(cudaStream_t st) {
+    if (beam_pending_ && !capturing(st)) cuda_check(cudaStreamWaitEvent(st, beam_done_, 0), "beam wait");
 }
 
 int Engine::check_device_error() {
@@ -549,6 +567,7 @@ bool Engine::fwd_begin(const BatchGeom& g, cudaStream_t st) {
     launches_cur_ = 0;
     if (g.n_utt == 0) { launches_last_ = 0; return false; }
     ensure_workspace(g);
+    wait_for_beam(st);
     upload_meta(g, st);
     if (g.M == 0) {
         cuda_check(cudaMemsetAsync(nspans_.p, 0, sizeof(int) * g.n_utt, st), "memset");

@@ -192,6 +192,11 @@ private:
     int held_n_utt_ = 0, held_T_max_ = 0;
     bool held_lost_ = false;
     DevBuf beam_state_;
+    // The last search may be on another stream than what comes next in its buffers (the state, the
+    // logits, the lengths): the next search and the next forward wait for it.
+    cudaEvent_t beam_done_ = nullptr;
+    bool beam_pending_ = false;
+    void wait_for_beam(cudaStream_t st);
     long long launches_cur_ = 0, launches_last_ = 0;
 
     // Captured forwards (CUDA graphs) of Engine::forward, keyed by the input
