@@ -135,3 +135,19 @@ def test_captured_search(B, model_path, synth):
     g.replay()
     assert same(a.host(), b.host())
     m.close()
+
+
+def test_closing_a_context_frees_the_search_state(B, model_path, synth):
+    """Contexts that have searched, opened and closed in turn (15 MB of beams each)."""
+    path = model_path("tiny", "q8_0", bias_std=0.02, gain_jitter=0.1)
+    d = torch.from_numpy(np.concatenate([synth.make_audio(160000, 1)] * 10)).cuda()
+    o = Outputs(10, 1, 8)
+    free = []
+    for _ in range(7):
+        m = B.Model(path)
+        m.forward_device(d.data_ptr(), [160000] * 10)
+        o.search(m, 128)
+        torch.cuda.synchronize()
+        m.close()
+        free.append(torch.cuda.mem_get_info()[0])
+    assert free[1] - free[-1] < 30 << 20, free

@@ -210,7 +210,8 @@ Engine::~Engine() {
     for (DevBuf* b : {&conv0_w_, &conv0_b_, &proj_lnw_, &proj_lnb_, &proj_w_.w, &proj_w_.s, &proj_b_, &pos_w_, &pos_b_,
                       &enc_lnw_, &enc_lnb_, &lm_w_.w, &lm_w_.s, &lm_b_, &audio_stage_, &meta_, &stats_, &gn_, &actA_,
                       &actB_, &feat_,
-                      &pbuf_, &x_, &xh_, &qkv_, &attn_, &hbuf_, &ybuf_, &lnstats_, &logits_, &ids_, &spans_, &nspans_, &err_})
+                      &pbuf_, &x_, &xh_, &qkv_, &attn_, &hbuf_, &ybuf_, &lnstats_, &logits_, &ids_, &spans_, &nspans_, &err_,
+                      &beam_state_})
         rel(*b);
     for (auto* v : {&conv_w_, &conv_b_, &conv_gw_, &conv_gb_})
         for (auto& b : *v) rel(b);
