@@ -802,14 +802,15 @@ __global__ void __launch_bounds__((NC + NP + 1) * 32, 1) ctc_beam_kernel(Params 
     for (int hi = s.n_nodes, lo; __syncthreads_or(left > 0) && hi > 0; hi = lo) {
         lo = max(hi - p.copied, 0);
         constexpr int kStep = kWarps * 32;
-        for (int k0 = lo + tid; k0 < hi; k0 += 8 * kStep) {
+        const int n = hi - lo;               // (counted from lo: node numbers go up to the end of an int)
+        for (int k0 = tid; k0 < n; k0 += 8 * kStep) {
             int2 v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (k0 + e * kStep < hi) v[e] = *reinterpret_cast<const int2*>(nodes + k0 + e * kStep);
+                if (k0 + e * kStep < n) v[e] = *reinterpret_cast<const int2*>(nodes + lo + k0 + e * kStep);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (k0 + e * kStep < hi) copy[k0 + e * kStep - lo] = v[e];
+                if (k0 + e * kStep < n) copy[k0 + e * kStep] = v[e];
         }
         __syncthreads();
         while (left > 0 && id >= lo && id < hi) {
