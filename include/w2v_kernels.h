@@ -220,8 +220,8 @@ int w2v_ctc_greedy(const float* logits, const long long* off, const int* T, int 
  *   workspace: device memory of w2v_lora_workspace_bytes(M, n_utt, rank)
  *      bytes, 128-byte aligned, not shared by calls that may overlap.
  *      W2V_ERR_CAPACITY when it is too small.
- * lora_b of an adapter in use must be finite: an infinity or NaN there may
- * reach the rows of other utterances nearby (at most 256 rows away).
+ * An infinity or NaN in an adapter stays with its utterances: those of their
+ * outputs that it takes part in are infinite or NaN, all others as without it.
  * A, W, lora_a, lora_b (and Bs) 16-byte aligned.  s_a lora_a[a] A[r] is held
  * as two fp16 numbers, value and remainder: to 2^-22 of it, and to no less than
  * 2^-25; its magnitude must stay below 65504. */

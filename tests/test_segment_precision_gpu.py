@@ -5,7 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_segment_gemm_gpu import EPI_F16, EPI_F16_GELU, EPI_F32, Lora, Segments, finish
+from test_segment_gemm_gpu import EPI_F16, EPI_F16_GELU, EPI_F32, EPI_F32_RESID, Lora, Segments, finish
 
 
 @pytest.fixture(scope="module")
@@ -45,3 +45,43 @@ def test_adapters_whose_ranks_cancel(K, synth, weights, epi, lens, rank):
         ref, tol = finish(t @ B.T, bound + (t.abs() * 2.0 ** -22 + 2.0 ** -25) @ B.abs().T, epi, None)
         d = (c.out[rows].double() - ref).abs()
         assert (d <= tol).all(), f"max error {d.max().item()} ({(d / tol).max().item()} of what is allowed)"
+
+
+@pytest.mark.parametrize("weights,N,Kd,rank,epi,lens", [
+    ("f16", 200, 128, 16, EPI_F16, [1] * 30), ("f16", 200, 128, 40, EPI_F32, [1] * 30), ("f16", 1024, 256, 8, EPI_F16_GELU, [300, 7, 260, 90]),
+    ("f16", 2304, 768, 64, EPI_F16, [499] * 5), ("f16", 93, 640, 24, EPI_F32_RESID, [70, 1, 200]), ("f16", 1024, 1088, 128, EPI_F32_RESID, [300] * 4),
+    ("q8", 200, 128, 16, EPI_F16, [1] * 30), ("q8", 93, 128, 40, EPI_F32, [1] * 30), ("q8", 1024, 256, 8, EPI_F16_GELU, [300, 7, 260, 90]),
+    ("q8", 1024, 1088, 64, EPI_F32_RESID, [499] * 5), ("q8", 94, 64, 24, EPI_F32_RESID, [70, 1, 200]), ("q8", 2304, 64, 8, EPI_F16, [700] * 40),
+    ("q4", 200, 128, 16, EPI_F16, [1] * 30), ("q4", 94, 128, 40, EPI_F32, [1] * 30), ("q4", 1024, 256, 128, EPI_F16_GELU, [300, 7, 260, 90]),
+    ("q4", 1024, 1088, 24, EPI_F32_RESID, [499] * 5)])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_an_infinite_adapter_stays_with_its_utterances(K, synth, weights, N, Kd, rank, epi, lens, value):
+    """An infinity or NaN in one adapter's second matrix: the outputs it belongs to (its utterances'
+    rows, its column) are no numbers, and every other output has the bits it has with a zero there."""
+    which = [(2 * i + 1) % 3 for i in range(len(lens))]
+    c = Lora(K, synth, Segments(lens), which, N, Kd, rank, 3, weights, epi)
+    places = [(0, rank - 1), (N - 1, 0), (N // 2, rank // 2)]
+    for n, k in places:
+        c.lb[1, n, k] = 0
+    c.call()
+    c.check()
+    clean = c.out.clone()
+    for n, k in places:
+        c.lb[1, n, k] = value
+    c.call()
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 0
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    for u, a in enumerate(which):
+        if a == 1:
+            for n, _ in places:
+                hit[c.seg.rows(u), n] = True
+    assert hit.any() and not hit.all()
+    bits = lambda t: t.view(torch.int16 if t.dtype == torch.float16 else torch.int32)
+    assert torch.equal(bits(c.out)[~hit], bits(clean)[~hit])
+    assert not torch.isfinite(c.out[hit]).any()
+    for n, k in places:                                    # and nothing of it is left in the next call
+        c.lb[1, n, k] = 0
+    c.call()
+    torch.cuda.synchronize()
+    assert torch.equal(bits(c.out), bits(clean))

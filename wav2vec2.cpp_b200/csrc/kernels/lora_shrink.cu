@@ -342,6 +342,11 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                 p.adapter[first_block + i] = slots[i];
             }
         }
+        if (blockIdx.y == 0 && warp * 32 < kRows) // this chunk's rows of each adapter
+            for (int s = 0; s < count; s++) {
+                const uint32_t mine = __ballot_sync(0xffffffffu, row_slot[tid] == s);
+                if (lane == 0) p.owners[(first_block + s) * kOwnerWords + local0 / 32 + warp] = mine;
+            }
         if (blockIdx.y == 0 && !direct)           // the others' blocks are zero in these rows
             for (int k = n_here; k < count; k++) {
                 __half* out = p.t + ((first_block + here[k]) * p.tile + local0) * t_columns(rank);

@@ -75,6 +75,7 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
     QLora<true> lo;
     lo.t = lo.b = m.x;
     lo.lora = n_utt > 0;
+    lo.lb = reinterpret_cast<const __half*>(lora_b);
     lo.plan = sg::lora_plan(workspace, M, n_utt, rank, rows);
     // as the fp16 kernel does (segment_gemm.cu): 512 of K, 1024 beside a residual
     lo.sum_blocks = epilogue == W2V_EPI_F32_RESID ? 16 : 8;

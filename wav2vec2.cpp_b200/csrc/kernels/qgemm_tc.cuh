@@ -41,6 +41,10 @@
 // boxes (same bytes per row: 32 ranks per k-block beside Q8_0 codes, 16 beside
 // Q4_0) and the converters copy them to tensor memory as they are; the value and the
 // remainder of the first product, both in the k-block's box, are multiplied by them in turn.
+// Activation rows are the MMA's columns, which have no mask, and a zero row of the block
+// times an infinity of the adapter would be no zero: the converters put zeros in the place
+// of what is not finite, say so, and the epilogue writes NaN where it belongs, in the
+// feature of that row for the adapter's own activation rows.
 #pragma once
 #include "segments.cuh"
 #include "w2v_kernels.h"
@@ -85,8 +89,12 @@ struct QLora<true> {
     sg::LoraPlan plan;
     int chunks;          // k-blocks per adapter
     int lora;            // the plan holds adapters
+    const __half* lb;    // what b maps
     int sum_blocks, n_sums;   // fp32 outputs: k-blocks of a sum, sums of a tile (segment_gemm.cu)
 };
+
+// Marks of the latest tiles with an adapter that is not finite: the tile's number + 1 (of this CTA's), by the number.
+constexpr int kSpoilt = 8;
 
 template <int BN, int WQ, bool PAIR, int EPI, int EH = 1>
 struct QCfg {
@@ -118,7 +126,9 @@ struct QCfg {
     static constexpr int kACol = 2 * BN;                        // first weight-tile column
     static_assert(kStages >= 2 && kSB >= 2, "plan");
     static_assert(kXBytes % 1024 == 0 && kCodeBytes % 1024 == 0, "alignment");
-    static_assert((3 * kStages + 2 * kSB + 5 + kNE * (kResBoxes > 1 ? kResBoxes : 1)) * 8 + 4 <= 512, "barriers");
+    static_assert((3 * kStages + 2 * kSB + 5 + kNE * (kResBoxes > 1 ? kResBoxes : 1)) * 8 + 4 + 4 * kSpoilt <= 512, "barriers");
+    // weight tiles that the converters may be ahead by, and the two accumulators
+    static_assert(kSB + 3 < kSpoilt, "tiles that are marked at once");
 };
 
 // ── tcgen05 forms used only here ────────────────────────────────────────────
@@ -204,6 +214,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
     constexpr int RB = Cfg::kResBoxes > 0 ? Cfg::kResBoxes : 1;
     uint64_t* rbar = done + 1;             // residual box b of epilogue warp w landed: rbar[RB w + b]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar + RB * kNE);
+    [[maybe_unused]] volatile int* spoilt = reinterpret_cast<int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -222,6 +233,8 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
         for (int b = 0; b < 2; b++) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], kNE * CT); }
         mbar_init(done, 1);
         for (int i = 0; i < RB * kNE; i++) mbar_init(&rbar[i], 1);
+        if constexpr (LORA)
+            for (int i = 0; i < kSpoilt; i++) spoilt[i] = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tmX);
         tma_prefetch_desc(&tmQ);
@@ -398,9 +411,9 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
         const int fl = 32 * q + lane;
         const uint32_t afull_lead = PAIR ? mapa_shared(smem_u32(afull), 0) : 0u;
         const uint32_t trow = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)Cfg::kACol;
-        int kq = 0;
+        int kq = 0, it = 0;
         bool ok = true;
-        for (int tile = unit; tile < total && ok; tile += n_units) {
+        for (int tile = unit; tile < total && ok; tile += n_units, it++) {
             int n_kb = p.k_blocks;
             for (int kb = 0; kb < n_kb; kb++, kq++) {
                 const int s = kq % S, f = kq % SB;
@@ -430,6 +443,16 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                             c = *reinterpret_cast<const uint4*>(
                                 row + ((j ^ (WQ == kQ8 ? (fl >> 1) & 3 : (fl >> 2) & 1)) << 4));
                         v[4 * j] = c.x; v[4 * j + 1] = c.y; v[4 * j + 2] = c.z; v[4 * j + 3] = c.w;
+                    }
+                    // an exponent of all ones carries into the sign's place
+                    auto odd = [](uint32_t x) { return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < 4 * kG; i++) any |= odd(v[i]);
+                    if (any) {
+#pragma unroll
+                        for (int i = 0; i < 4 * kG; i++) v[i] &= ~((odd(v[i]) >> 15) * 0xffffu);
+                        spoilt[it % kSpoilt] = it + 1;
                     }
                 } else if constexpr (WQ == kQ8) {
                     // 64-byte rows, 64-byte swizzle: 16-byte group j at j ^ ((row >> 1) & 3)
@@ -512,6 +535,31 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
             tacc = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(ab * BN);
             return true;
         };
+        // NaN in feature f of the chunk's rows whose adapter has something that is not finite there.
+        [[maybe_unused]] auto spoil = [&](float (&v)[32], int ri, int c, int f) {
+            if constexpr (LORA) {
+                sg::grid_dependency_wait();
+                const sg::LoraTile& lt = lo.plan.tiles[ri];
+                const int first = lt.first, count = lt.count;
+#pragma unroll 1
+                for (int blk = first; blk < first + count; blk++) {
+                    const uint32_t rows = lo.plan.owners[(long long)blk * sg::kOwnerWords + c];
+                    bool odd = false;
+                    if (rows && f < p.N) {
+                        const uint32_t* row = reinterpret_cast<const uint32_t*>(lo.lb + ((long long)lo.plan.adapter[blk] * p.N + f) * lo.plan.rank);
+#pragma unroll 1
+                        for (int i = 0; i < lo.plan.rank / 2; i++) odd = odd || (((row[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (odd && (rows >> j & 1u)) v[j] = __int_as_float(0x7fffffff);
+                }
+            }
+        };
+        auto is_spoilt = [&](int it) {
+            if constexpr (LORA) return spoilt[it % kSpoilt] == it + 1;
+            else return false;
+        };
         if (p.tma) {
             // Staged: per 32 x 32 chunk, the residual box arrives by TMA R - 1 chunks
             // ahead (a ring of R boxes per warp, the first R - 1 requested before the
@@ -578,6 +626,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                     stn = p.ln_stats[ri * BN + eh * 32 + lane];
                 uint32_t tacc;
                 if (!take(ab, aph, tempty_lead, tacc)) break;
+                const bool spoils = is_spoilt(it);
                 bool ok = true;
 #pragma unroll 1
                 for (int c = eh, k = 0; c < kNch; c += EH, k++) {
@@ -594,6 +643,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                     }
                     const int r0 = ri * BN + c * 32;
                     if (r0 >= p.m_valid) continue;
+                    if (spoils) spoil(v, ri, c, fcol);
                     const float2 st = stn;
                     if (EPI == W2V_EPI_F32_RESID_LN && c + EH < kNch)
                         stn = r0 + 32 * EH + lane < p.m_valid ? p.ln_stats[r0 + 32 * EH + lane] : make_float2(0.f, 0.f);
@@ -693,6 +743,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
             if (kRes) fetch(eh);
             uint32_t tacc;
             if (!take(ab, aph, tempty_lead, tacc)) break;
+            const bool spoils = is_spoilt(it);
 #pragma unroll 1
             for (int c = eh; c < kNch; c += EH) {
                 float v[32];
@@ -715,6 +766,7 @@ qgemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CU
                     if (c + EH < kNch && r0 + 32 * EH < p.m_valid) fetch(c + EH);
                 }
                 if (r0 >= p.m_valid) continue;
+                if (spoils) spoil(v, ri, c, fcol);
                 if (EPI == W2V_EPI_F16 || EPI == W2V_EPI_F16_GELU) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {

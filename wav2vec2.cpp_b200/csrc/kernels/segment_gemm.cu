@@ -52,11 +52,13 @@ constexpr int kNE = 8;                         // epilogue warps
 constexpr int kThreads = 64 + 32 * kNE;
 constexpr int kSmemCap = 232448;
 constexpr int kABytes = kBM * kBK * 2;
+constexpr int kTailBytes = 512;                // barriers, the stages' work
 constexpr int kEpiBytes = kNE * 4096;          // per warp: a 32 x 32 fp32 chunk, or two fp16 store boxes
 constexpr int kMaxStages = 8;
 // A stage's work: its number of MMA steps, these, and a mask from kWrap on: step k takes columns 16 k of
 // the rows and 16 (k & mask) of the weights (an adapter's value and remainder meet the same ones).
-constexpr uint32_t kLastOfTile = 16, kLastOfSum = 32, kWrap = 8, kMainWork = kBK / 16 | (kBK / 16 - 1) << kWrap;
+// kOwned: an adapter's, whose product changes its own rows only.
+constexpr uint32_t kLastOfTile = 16, kLastOfSum = 32, kOwned = 64, kWrap = 8, kMainWork = kBK / 16 | (kBK / 16 - 1) << kWrap;
 __host__ __device__ constexpr bool sums_of(int epi) { return epi == W2V_EPI_F32 || epi == W2V_EPI_F32_RESID; }
 // K-blocks of a sum: 512 of K; beside a residual, which as a rule is larger than what is added to it, 1024.
 __host__ __device__ constexpr int sum_blocks(int epi) { return epi == W2V_EPI_F32_RESID ? 16 : 8; }
@@ -300,6 +302,8 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     uint32_t* stage_work = tmem_slot + 1;      // what the MMA does with a stage
+    uint32_t* stage_off = reinterpret_cast<uint32_t*>(epi + kEpiBytes + 256);   // an adapter's: the rows left alone
+    static_assert((2 * kMaxStages + 5) * 8 + 4 + 4 * kMaxStages <= 256 && 256 + kMaxStages * kOwnerWords * 4 <= kTailBytes, "tail");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -357,13 +361,17 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // grouped: of the rows only the 32-row boxes that hold valid ones, where that saves any (tmT, which is
         // theirs then): what the MMA reads in the others' places goes to accumulator rows that are not stored
         int boxes = 4;
+        // owners of four of the tile's blocks, a word per lane, and which of the four the stage's is
+        uint32_t owners = 0;
+        int owner_at = 0;
         // k, kw: first column of the rows' and of the weights' tile
         auto stage_in = [&](const CUtensorMap* ma, const CUtensorMap* mb, int k, int ra, int rb, int gb, uint32_t work, int kw) {
             if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.err)) { ok = false; return; }
             const uint32_t dst = base + (uint32_t)(stage * stage_bytes), bar = full_lead + (uint32_t)(stage * 8);
             if (WORK && lane == 0) stage_work[stage] = work;
-            if (WORK) __syncwarp();
-            expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
+            const bool owned = LORA && (work & kOwned);
+            if (WORK && !owned) __syncwarp();
+            if (!owned) expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
             if (LORA || boxes == 4) {
                 tma_load_2d_if<PAIR>(lead, dst, ma, bar, k, ra + (int)rank * kBM);
             } else {
@@ -371,6 +379,11 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tma_load_2d_if<PAIR>(lead, dst + (uint32_t)(i * kABytes / 4), &tmT, bar, k, ra + (int)rank * kBM + i * 32);
             }
             tma_load_3d_if<PAIR>(lead, dst + kABytes, mb, bar, kw, rb + b_row, gb);
+            if (owned) {                       // (behind the loads: the owners may still be on their way)
+                if (lane / kOwnerWords == owner_at) stage_off[stage * kOwnerWords + lane % kOwnerWords] = ~owners;
+                __syncwarp();
+                expect_tx_if(arm, smem_u32(&full[stage]), arm_bytes);
+            }
             issued |= 1u << stage;
             last_par = (last_par & ~(1u << stage)) | (phase << stage);
             if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -397,16 +410,22 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 first = uniform(__shfl_sync(0xffffffffu, rec, 0));
                 blocks = uniform(__shfl_sync(0xffffffffu, rec, 1));
             }
+            auto owners_from = [&](int b) {
+                if (b + lane / kOwnerWords < blocks) owners = p.plan.owners[(long long)(first + b) * kOwnerWords + lane];
+            };
+            owners_from(0);
             if (ok)
                 stage_in(&tmA, &tmB, (p.k_blocks - 1) * kBK, t.row0, col0, t.group, kMainWork | (blocks ? 0 : kLastOfTile | kLastOfSum), (p.k_blocks - 1) * kBK);
             for (int b = 0; b < blocks && ok; b++) {
                 const int held = __shfl_sync(0xffffffffu, rec, min(2 + b, 31));
                 const int ad = uniform(b < kInline ? held : p.plan.adapter[first + b]);
+                owner_at = b % (32 / kOwnerWords);
+                if (b && owner_at == 0) owners_from(b);
                 for (int c = 0; c < chunks && ok; c++) {
                     const uint32_t steps = (uint32_t)group_width(p.plan.rank, c * kGroup) / 16;
                     const bool last = b + 1 == blocks && c + 1 == chunks;
                     stage_in(&tmT, &tmL, c * kBK, (first + b) * kTileRows, col0, ad,
-                             2 * steps | (steps - 1) << kWrap | (last ? kLastOfTile | kLastOfSum : 0), c * kGroup);
+                             kOwned | 2 * steps | (steps - 1) << kWrap | (last ? kLastOfTile | kLastOfSum : 0), c * kGroup);
                 }
             }
         }
@@ -437,9 +456,9 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tc_fence_after();
                     return true;
                 };
-                auto multiply = [&](uint32_t go, int kk, int kw) {
+                auto multiply = [&](uint32_t go, int kk) {
                     const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
-                    umma_f16_if<PAIR>(go, d, desc_plus(da, kk * 32), desc_plus(db, kw * 32), idesc, !first || kk != 0);
+                    umma_f16_if<PAIR>(go, d, desc_plus(da, kk * 32), desc_plus(db, kk * 32), idesc, !first || kk != 0);
                 };
                 auto end = [&](bool last_of_sum) {
                     umma_commit_if<PAIR>(lead, empty_here + (uint32_t)(stage * 8));
@@ -457,16 +476,26 @@ seg_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 for (int kb = 0; kb < p.k_blocks - 1; kb++) {
                     if (!begin()) { ok = false; break; }
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; kk++) multiply(lead, kk, kk);
+                    for (int kk = 0; kk < kBK / 16; kk++) multiply(lead, kk);
                     end(SUMS && kb % sum_blocks(EPI) == sum_blocks(EPI) - 1);
                 }
                 // the last of K and the adapters' stages: as the producer found them
                 for (uint32_t work = 0; ok && !(work & kLastOfTile);) {
                     if (!begin()) { ok = false; break; }
                     work = WORK ? (uint32_t)uniform((int)stage_work[stage]) : kMainWork | kLastOfSum | kLastOfTile;
+                    if (LORA && (work & kOwned)) {
+                        const uint4* words = reinterpret_cast<const uint4*>(stage_off + stage * kOwnerWords);
+                        const uint4 o0 = words[0], o1 = words[PAIR ? 1 : 0];
+                        const uint32_t off[kOwnerWords] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+                        const uint64_t da = desc_plus(desc0, (uint32_t)(stage * stage_bytes)), db = desc_plus(da, kABytes);
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; kk++)
-                        multiply(LORA ? lead & (uint32_t)(kk < (int)(work & 15u)) : lead, kk, LORA ? kk & (int)(work >> kWrap) : kk);
+                        for (int kk = 0; kk < kBK / 16; kk++)
+                            umma_f16_masked_if<PAIR>(lead & (uint32_t)(kk < (int)(work & 15u)), d, desc_plus(da, kk * 32),
+                                                     desc_plus(db, (kk & (int)(work >> kWrap)) * 32), idesc, off);
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < kBK / 16; kk++) multiply(lead, kk);
+                    }
                     end((work & kLastOfSum) != 0);
                 }
             }
@@ -688,7 +717,7 @@ static int common(const Call& c, bool lora, int bn, bool pair, Params& p, Maps& 
     p.bn = bn;
     p.n_tiles = (c.N + bn - 1) / bn;
     p.b_bytes = (pair ? bn / 2 : bn) * kBK * 2;
-    p.stages = std::min(kMaxStages, (kSmemCap - 1024 - 256 - kEpiBytes) / (kABytes + p.b_bytes));
+    p.stages = std::min(kMaxStages, (kSmemCap - 1024 - kTailBytes - kEpiBytes) / (kABytes + p.b_bytes));
     p.vec = c.ldc % 4 == 0 && C % (f16 ? 8 : 16) == 0 &&
             (c.epilogue != W2V_EPI_F32_RESID || (c.ldr % 4 == 0 && R % 16 == 0));
     p.bias_vec = reinterpret_cast<uintptr_t>(c.bias) % 16 == 0 && (c.n_mats == 1 || c.N % 4 == 0);

@@ -19,6 +19,10 @@ namespace sg {
 // 32 ranks of the one, then of the other, so that both meet the same columns of B within
 // one K-block: a row is groups of 64 columns, the last of 2 w where w = 16 or 32 ranks
 // are left (the rank rounded up to 16; zero behind it).
+//
+// A zero row times an infinity is no zero, so the blocks' zeros alone would let what one
+// adapter's B holds reach every row of the tile: the block's owners are the rows that its
+// product may change.
 // Tile i's blocks are first .. first + count - 1 with
 //   first = i + min(utterances that end before the tile, rows before it),
 // which leaves room for every tile without a scan over the tiles before: of a
@@ -31,6 +35,7 @@ struct LoraTile {          // 64 bytes: one load of half a warp
 struct LoraPlan {
     LoraTile* tiles;       // [row tiles]
     int* adapter;          // [blocks]
+    uint32_t* owners;      // [blocks][kOwnerWords]: bit r % 32 of word r / 32, row r of the tile is this adapter's
     __half* t;             // [blocks][tile][t_columns(rank)]
     int tile;              // rows per tile: 64, 128, 192 or 256
     int rank;
@@ -61,11 +66,13 @@ __host__ __device__ inline int group_width(int rank, int r) { return rank16(rank
 __host__ inline long long lora_blocks(long long M, int n_utt, int tile) {
     return (M + tile - 1) / tile + (n_utt < M ? n_utt : M);
 }
+constexpr int kOwnerWords = 8;               // 256 rows
 // Workspace for any tile height; lora_plan lays one height's plan out in it.
 __host__ inline long long lora_workspace(long long M, int n_utt, int rank) {
     const long long rows = M + 256 * (1 + (n_utt < M ? n_utt : M));
-    const long long tiles = M / 64 + 1;
-    return (tiles * (long long)sizeof(LoraTile) + 255) / 256 * 256 + ((tiles + (n_utt < M ? n_utt : M)) * 4 + 255) / 256 * 256 + rows * t_columns(rank) * 2 + 256;
+    const long long tiles = M / 64 + 1, blocks = tiles + (n_utt < M ? n_utt : M);
+    return (tiles * (long long)sizeof(LoraTile) + 255) / 256 * 256 + (blocks * 4 + 255) / 256 * 256 +
+           (blocks * kOwnerWords * 4 + 255) / 256 * 256 + rows * t_columns(rank) * 2 + 256;
 }
 __host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, int tile) {
     LoraPlan p;
@@ -77,6 +84,8 @@ __host__ inline LoraPlan lora_plan(void* ws, long long M, int n_utt, int rank, i
     at += ((M + tile - 1) / tile * (long long)sizeof(LoraTile) + 255) / 256 * 256;
     p.adapter = reinterpret_cast<int*>(at);
     at += (p.blocks * 4 + 255) / 256 * 256;
+    p.owners = reinterpret_cast<uint32_t*>(at);
+    at += (p.blocks * kOwnerWords * 4 + 255) / 256 * 256;
     p.t = reinterpret_cast<__half*>(at);
     return p;
 }
@@ -137,6 +146,25 @@ W2V_DEV void umma_f16_if(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64
             "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
             " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
             "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+            : "memory");
+}
+// The same, leaving the rows (TMEM lanes) whose bit is set as they are: words 0 .. 3 those of this
+// CTA (the first of a pair), 4 .. 7 of the second.
+template <bool PAIR>
+W2V_DEV void umma_f16_masked_if(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                const uint32_t (&off)[kOwnerWords]) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.eq.b32 p, 0, 0;\n setp.ne.b32 q, %4, 0;\n"
+            " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(lead), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
+            "r"(off[5]), "r"(off[6]), "r"(off[7])
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.eq.b32 p, 0, 0;\n setp.ne.b32 q, %4, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(lead), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
             : "memory");
 }
 // bar: shared::cluster address
