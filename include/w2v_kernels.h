@@ -218,7 +218,8 @@ int w2v_ctc_greedy(const float* logits, const long long* off, const int* T, int 
  *   off, T, adapter: device arrays of n_utt entries; off[u+1] >= off[u] + T[u],
  *      T[u] <= 0 is an utterance without rows.  n_utt == 0: no adapters.
  *   workspace: device memory of w2v_lora_workspace_bytes(M, n_utt, rank)
- *      bytes, 128-byte aligned, not shared by calls that may overlap.
+ *      bytes (-1: sizes that the calls refuse, M + 256 (1 + min(n_utt, M)) past
+ *      2^31 - 1 among them), 128-byte aligned, not shared by calls that may overlap.
  *      W2V_ERR_CAPACITY when it is too small.
  * An infinity or NaN in an adapter stays with its utterances: those of their
  * outputs that it takes part in are infinite or NaN, all others as without it.

@@ -114,3 +114,16 @@ def test_bytes_that_pass_64_bits_are_refused(L):
     assert per > 0 and per * n > (1 << 63) - 1               # (a product of 64 bits would be another number)
     assert L.w2v_ctc_beam_state_bytes(n, 32, 128, 16000000) == -1
     assert beam(L, n_utt=n, width=128, max_frames=16000000, state_bytes=(1 << 63) - 1) == ARGS
+
+
+@pytest.mark.parametrize("f", [lora, lora_q])
+def test_a_workspace_size_is_given_for_what_the_calls_take(L, f):
+    """Single rows by the million: up to M + 256 (1 + min(n_utt, M)) = 2^31 - 1 there is a size and the
+    calls want that much; past it there is none and they are refused."""
+    for rows in (8000000, 8355966):            # 257 rows + 256 <= 2^31 - 1
+        need = L.w2v_lora_workspace_bytes(rows, rows, 8)
+        assert need > 0 and f(L, M=rows, n_utt=rows, rank=8, ws_bytes=need - 1) == CAPACITY
+    for rows in (8355967, 9000000, 100000000):
+        assert L.w2v_lora_workspace_bytes(rows, rows, 8) == -1
+        assert f(L, M=rows, n_utt=rows, rank=8, ws_bytes=1 << 60) == ARGS
+    assert L.w2v_lora_workspace_bytes(2000000000, 3, 8) > 0

@@ -61,7 +61,10 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
     if (M == 0 && K > 0 && K % kBK == 0 && N > 0 && ldc >= N) return W2V_OK;
     if (n_utt > 0 && (!off || !T || !adapter)) return W2V_ERR_ARGS;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 127)) return W2V_ERR_ARGS;
-    if (M >= 0 && workspace_bytes < sg::lora_workspace(M, n_utt, rank)) return W2V_ERR_CAPACITY;
+    if (M < 0) return W2V_ERR_ARGS;
+    const long long need = sg::lora_workspace(M, n_utt, rank);
+    if (need < 0) return W2V_ERR_ARGS;
+    if (workspace_bytes < need) return W2V_ERR_CAPACITY;
     QParams p;
     QMaps m;
     int bn = 0;
@@ -82,7 +85,6 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
     lo.n_sums = f16 ? 1 : (int)((K / kBK + lo.sum_blocks - 1) / lo.sum_blocks);
     lo.chunks = (2 * rank + code_row_bytes(wq) - 1) / code_row_bytes(wq);
     if (lo.lora) {
-        if (lo.plan.blocks * rows > 0x7fffffffLL) return W2V_ERR_ARGS;
         auto enc = get_encode();
         const uint32_t es[3] = {1, 1, 1};
         const uint64_t td[2] = {(uint64_t)sg::t_columns(rank), (uint64_t)(lo.plan.blocks * rows)};

@@ -774,7 +774,9 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
         return W2V_ERR_ARGS;
     if (M == 0) return W2V_OK;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 127)) return W2V_ERR_ARGS;
-    if (workspace_bytes < lora_workspace(M, n_utt, rank)) return W2V_ERR_CAPACITY;
+    const long long need = lora_workspace(M, n_utt, rank);
+    if (need < 0) return W2V_ERR_ARGS;
+    if (workspace_bytes < need) return W2V_ERR_CAPACITY;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     Params p = {};
     Maps m;
@@ -788,7 +790,6 @@ extern "C" int w2v_gemm_f16_lora(const void* A, long long lda, long long K, long
     p.lora = n_utt > 0;
     p.plan = lora_plan(workspace, M, n_utt, rank, tile_rows);
     if (p.lora) {
-        if (p.plan.blocks * tile_rows > 0x7fffffffLL) return W2V_ERR_ARGS;
         const uint64_t td[2] = {(uint64_t)t_columns(rank), (uint64_t)(p.plan.blocks * tile_rows)};
         const uint64_t ts[1] = {(uint64_t)t_columns(rank) * 2};
         rc = map_f16(&m.t, p.plan.t, 2, td, ts, p.a_rows);

@@ -67,9 +67,11 @@ __host__ inline long long lora_blocks(long long M, int n_utt, int tile) {
     return (M + tile - 1) / tile + (n_utt < M ? n_utt : M);
 }
 constexpr int kOwnerWords = 8;               // 256 rows
-// Workspace for any tile height; lora_plan lays one height's plan out in it.
+// Workspace for any tile height; lora_plan lays one height's plan out in it.  -1: more rows
+// of blocks than an int numbers (the TMA's coordinate).
 __host__ inline long long lora_workspace(long long M, int n_utt, int rank) {
     const long long rows = M + 256 * (1 + (n_utt < M ? n_utt : M));
+    if (rows > 0x7fffffffLL) return -1;
     const long long tiles = M / 64 + 1, blocks = tiles + (n_utt < M ? n_utt : M);
     return (tiles * (long long)sizeof(LoraTile) + 255) / 256 * 256 + (blocks * 4 + 255) / 256 * 256 +
            (blocks * kOwnerWords * 4 + 255) / 256 * 256 + rows * t_columns(rank) * 2 + 256;
