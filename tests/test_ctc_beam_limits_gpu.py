@@ -46,3 +46,30 @@ def test_nodes_up_to_the_end_of_an_int(K):
     assert b.results() == [[]] and int(b.err.item()) == 2
     del b
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("V,width", [(40, 5), (33, 32), (94, 33), (94, 100), (192, 9), (193, 9), (200, 100), (400, 20), (400, 128), (1024, 31), (1024, 127)])
+def test_tokens_of_equal_probability(K, V, width):
+    """Logits on a coarse grid, as 16-bit heads and masked tokens of one value give: single frames,
+    whose hypotheses in order are the tokens by value and then by id, the blank's (nothing) before
+    tokens as likely as it."""
+    rng = np.random.default_rng(V + width)
+    logits = [(np.round(rng.standard_normal((1, V)) * 2) / g).astype(np.float32) for g in (1, 4, 64)]
+    logits += [np.zeros((1, V), np.float32), np.where(rng.random((1, V)) < 0.05, 1.0, -8.0).astype(np.float32)]
+    close = np.full((1, V), -1.0, np.float32)         # neighbours of a number: the same leading bits, other values
+    close[0, ::3] = np.nextafter(np.float32(-1), np.float32(0))
+    logits.append(close)
+    b = Beam(K, logits, 3, width, width)
+    b.call()
+    b.check(logits)
+
+
+@pytest.mark.parametrize("V,width", [(94, 20), (200, 34), (1024, 6)])
+def test_paths_of_equal_probability_among_many_tokens(K, V, width):
+    """Rows of 0 and -inf: whole numbers of paths, most of them equal."""
+    rng = np.random.default_rng(V)
+    lg = np.where(rng.random((7, V)) < 0.4, 0.0, -np.inf).astype(np.float32)
+    lg[np.arange(7), rng.integers(0, V, 7)] = 0.0
+    b = Beam(K, [lg], 0, width, width)
+    b.call()
+    b.check([lg], counts=True)

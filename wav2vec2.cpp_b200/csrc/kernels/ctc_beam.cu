@@ -194,7 +194,7 @@ W2V_DEV uint32_t leading(u64 k) { return (uint32_t)((k - kLeast) >> 30); }
 
 // Row producer: one warp turns the logits of a frame into a Row.  Tokens are
 // ranked by how many have larger leading bits, four keys a load; where two have
-// the same (one frame in a thousand), by the whole values and the id.  Of a large
+// the same, once more with the whole values and the id.  Of a large
 // vocabulary only those are looked at that can be among the first n_tok: with m
 // of a lane's tokens at or above the least m-th largest of all lanes, 32 m are.
 template <bool LARGE>     // vocabularies of more than 64
@@ -263,16 +263,44 @@ W2V_DEV void make_row(const float* x, int V, int blank, int n_tok, float mx, con
     }
     ranks = __reduce_add_sync(0xffffffffu, ranks);
     some = __reduce_add_sync(0xffffffffu, some);
-    if (ranks != some * (some - 1) / 2)
-        for (int v = lane; v < V; v += 32) {
-            const u64 e = bits_of(r.p[v]);
-            int rank = 0;
-            for (int w = 0; w < V; w++) {
-                const u64 f = bits_of(r.p[w]);
-                rank += w != blank && (w < v ? f >= e : f > e);
+    if (ranks != some * (some - 1) / 2) {
+        // Among the same keys by the whole values and the id (the list's order).  Logits that came
+        // from 16 bits, or that share a masked token's value, are here in nearly every frame.  Of
+        // few tokens all values are compared, without a branch (32, 24 of them masked: 1.6 us a frame,
+        // by the keys 1.9); of many by the keys, until n_tok are found to be better (400 tokens from
+        // 16 bits, width 8: 4.5 us a frame, 1024: 7.3; by the values of all tokens 36 and 219).
+        __syncwarp();
+        if (!LARGE)
+            for (int v = lane; v < V; v += 32) {
+                const u64 e = bits_of(r.p[v]);
+                int rank = 0;
+                for (int w = 0; w < V; w++) {
+                    const u64 f = bits_of(r.p[w]);
+                    rank += w != blank && (w < v ? f >= e : f > e);
+                }
+                if (v != blank && rank < n_tok) r.by_rank[rank] = Ranked{value_of(e), v, 0};
             }
-            if (v != blank && rank < n_tok) r.by_rank[rank] = Ranked{value_of(e), v, 0};
+        else for (int a = lane; a < n; a += 32) {
+            const uint32_t k = r.key[a];
+            if (!k) continue;
+            const int v = some_only ? r.id[a] : a;
+            const double e = r.p[v];
+            int rank = 0;
+            for (int w = 0; w < n4 && rank < n_tok; w++) {
+                const uint4 q = reinterpret_cast<const uint4*>(r.key)[w];
+                rank += (q.x > k) + (q.y > k) + (q.z > k) + (q.w > k);
+                const uint32_t same[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (same[i] == k) {
+                        const int b = 4 * w + i;
+                        const double f = r.p[some_only ? r.id[b] : b];
+                        rank += b < a ? f >= e : f > e;
+                    }
+            }
+            if (rank < n_tok) r.by_rank[rank] = Ranked{e, v, 0};
         }
+    }
     if (lane == 0) *r.z = z;
     __syncwarp();
 }
