@@ -85,3 +85,68 @@ def test_an_infinite_adapter_stays_with_its_utterances(K, synth, weights, N, Kd,
     c.call()
     torch.cuda.synchronize()
     assert torch.equal(bits(c.out), bits(clean))
+
+
+def rms(got, ref):
+    return float(((got.double() - ref) ** 2).sum().sqrt() / (ref ** 2).sum().sqrt())
+
+
+# Relative error (root mean square) of fp32 outputs.  A tensor core's running sum is cut towards zero
+# behind its 24th bit at each 16 products; on normal inputs that is 1.1e-6, 2.3e-6, 4.5e-6 and 5.6e-6 of
+# the result over K 1024, 2112, 4096 and 5120 in one sum, and 5.8e-7 at any K where the sums end every
+# 512; beside a residual of twice the size 6.5e-7, 1.3e-6, 2.6e-6 and 3.3e-6, and 6.5e-7 where they end
+# every 1024 (simulated in 64 bits).  The bound lies between the two.
+NEAR = {EPI_F32: 8e-7, EPI_F32_RESID: 9e-7}
+
+
+@pytest.mark.parametrize("weights", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_F32_RESID])
+@pytest.mark.parametrize("Kd,rank", [(1024, 16), (2112, 16), (4096, 16), (5120, 16), (2112, 128), (5120, 128), (4096, 72)])
+def test_adapters_long_sums_keep_their_bits(K, synth, weights, epi, Kd, rank):
+    c = Lora(K, synth, Segments([130, 0, 1, 300]), [1, 0, 0, 2], 1024, Kd, rank, 3, weights, epi)
+    c.call()
+    c.check()
+    ref = c.x.double() @ c.w.double().T + c.bias.double()
+    for u, a in enumerate([1, 0, 0, 2]):
+        rows = c.seg.rows(u)
+        ref[rows] += (c.x[rows].double() @ c.la[a].double().T * float(c.scale[a].double())) @ c.lb[a].double().T
+    if epi == EPI_F32_RESID:
+        ref += c.resid0.double()
+    assert rms(c.out[:c.seg.M], ref) < NEAR[epi]
+
+
+@pytest.mark.parametrize("epi", [EPI_F32, EPI_F32_RESID])
+@pytest.mark.parametrize("N,Kd", [(200, 1024), (200, 2112), (48, 4096), (1024, 5120)])
+def test_grouped_long_sums_keep_their_bits(K, epi, N, Kd):
+    g = torch.Generator(device="cuda").manual_seed(N + Kd)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    seg, group = Segments([130, 0, 1, 300]), [1, 0, 0, 2]
+    x, w, b, resid = r(seg.M, Kd).half(), (r(3, N, Kd) / Kd ** 0.5).half(), r(3, N), 2 * r(seg.M, N)
+    out, err = torch.empty(seg.M, N, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    which = torch.tensor(group, dtype=torch.int32, device="cuda")
+    K.gemm_grouped(x.data_ptr(), Kd, Kd, seg.M, w.data_ptr(), 3, N, out.data_ptr(), N, b.data_ptr(), resid.data_ptr(), N, epi,
+                   seg.off.data_ptr(), seg.T.data_ptr(), which.data_ptr(), 4, err.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    ref = torch.cat([x[seg.rows(u)].double() @ w[e].double().T + b[e].double() for u, e in enumerate(group)])
+    if epi == EPI_F32_RESID:
+        ref += resid.double()
+    assert rms(out, ref) < NEAR[epi]
+
+
+@pytest.mark.parametrize("weights", ["f16", "q8"])
+@pytest.mark.parametrize("epi", [EPI_F16, EPI_F32])
+@pytest.mark.parametrize("M,n_adapters", [(64, 32), (64, 33), (65, 16), (65, 17), (128, 16), (128, 17), (129, 10), (129, 11)])
+def test_both_sides_of_a_block_per_adapter(K, synth, weights, epi, M, n_adapters):
+    """The first product gives each adapter blocks of its own while the 64-row blocks times the
+    adapters are 32 or fewer: products of 32 and just past it, adapters that no row uses among
+    them, all adapters in the last block's single row's neighbourhood or none."""
+    lens = [1] * 20 + [M - 41, 1] + [1] * 20
+    which = [(7 * i) % n_adapters if i % 5 else -1 for i in range(len(lens))]
+    which = [a if a != 3 else 4 for a in which]                       # adapter 3: no row's
+    c = Lora(K, synth, Segments(lens), which, 200, 192, 16, n_adapters, weights, epi)
+    assert c.seg.M == M
+    c.la[3].fill_(float("nan"))
+    c.lb[3].fill_(float("inf"))
+    c.call()
+    c.check()

@@ -20,6 +20,10 @@
 // Each takes every fourth stage into accumulators of its own, which are added when
 // they are read.
 //
+// Sums over K: for fp32 outputs an issuer's end every 512 of its K, as the projection's do
+// (segment_gemm.cu says why); the planning warps then add them to totals with columns of their own,
+// and the issuers wait until that is done.  Up to K = 2048 (rank 32 and below) there is one sum.
+//
 // Few rows (kDirect): what counts is the way from the launch to the results.
 // Each adapter has a block of its own whether the rows use it or not, which loads and
 // multiplies before the plan is there.  Projections with adapters, the whole call
@@ -34,6 +38,7 @@ namespace sg {
 constexpr int kStep = 64, kMaxTile = 256;
 constexpr int kPlanners = 128, kProducer = kPlanners / 32, kIssuers = 4, kThreads = kPlanners + 32 + 32 * kIssuers;
 constexpr int kMaxRing = 8;
+constexpr int kSumSteps = 512 / kStep;         // K-steps of a sum
 // Blocks up to which each adapter has its own: up to 32 the call gains 0.6 to 1.8 us (of 10 to 24);
 // at 64 some gain 0.2 to 1.0, others lose 1.9 to 2.5, the blocks standing where the projection's would start.
 constexpr int kDirect = 32;
@@ -41,11 +46,12 @@ constexpr int kDirect = 32;
 struct ShrinkShape {
     int stages, stage_bytes, smem, cols;       // cols: of TMEM
     int issuers;                               // warps that multiply
+    int sums;                                  // of an issuer's over K
     int direct;                                // block y takes adapter y, used or not
     int x_bytes;                               // of a box of x
 };
 // Two blocks per SM where a ring of three stages or more allows it.
-static ShrinkShape shrink_shape(int rows, int rank) {
+static ShrinkShape shrink_shape(int rows, int rank, int k_steps, bool sums) {
     ShrinkShape s;
     s.stage_bytes = (rows + 2 * rank) * kStep * 2;
     const int behind = 64 * kStep * 2 + 1024;  // what the last stage's MMAs may read past it
@@ -56,10 +62,25 @@ static ShrinkShape shrink_shape(int rows, int rank) {
     s.smem = 1024 + s.stages * s.stage_bytes + behind + 256;
     const int acc = 2 * ((rank + 15) / 16 * 16);
     s.issuers = kIssuers;
-    while (s.issuers > 1 && (s.issuers * acc > 256 || s.stages % s.issuers)) s.issuers /= 2;
+    auto n_sums = [&] { return sums ? (k_steps + kSumSteps * s.issuers - 1) / (kSumSteps * s.issuers) : 1; };
+    auto columns = [&] { return (s.issuers + (n_sums() > 1 ? 1 : 0)) * acc; };
+    while (s.issuers > 1 && (columns() > 256 || s.stages % s.issuers)) s.issuers /= 2;
+    s.sums = n_sums();
     s.cols = 32;
-    while (s.cols < s.issuers * acc) s.cols *= 2;
+    while (s.cols < columns()) s.cols *= 2;    // (at most 256 and the totals' 256)
     return s;
+}
+
+// 16 columns of TMEM of this warp's lanes <- 16 registers.
+W2V_DEV void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+        "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+        "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+        "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
+        : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // Barriers of the four warps that plan.
@@ -106,7 +127,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const bool direct = shape.direct != 0;
     // the block that is sure to use its rows fetches the first of them before it knows the adapters
     const int early = blockIdx.y == 0 && !direct ? min(S, k_steps) : 0;
-    const int issuers = shape.issuers, acc_cols = 2 * n16;
+    const int issuers = shape.issuers, acc_cols = 2 * n16, sums = shape.sums;
+    const int sum_steps = sums > 1 ? kSumSteps * issuers : k_steps;       // of all issuers
 
     // a stage's x and the adapters' share complete on full[st]
     const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), lead = elect_one();
@@ -136,29 +158,31 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     auto multiply = [&](int n, int pass) {
         const int w = warp - kProducer - 1;
         if (w >= issuers) return;
-        if (pass > 0 && ok && !mbar_wait_warp(&drained, (uint32_t)(pass - 1) & 1u, a.err)) ok = false;
-        tc_fence_after();
         const uint32_t idesc = umma_idesc_f16(128, n16), d0 = (uint32_t)uniform((int)tmem_slot) + (uint32_t)(w * acc_cols);
         const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
         int at = st + w;
         uint32_t par = odd;
         if (at >= S) { at -= S; par ^= 1u; }
-        for (int ks = w; ks < k_steps && ok; ks += issuers) {
-            if (!mbar_wait_warp(&full[at], par, a.err)) { ok = false; break; }
+        for (int ks0 = 0, sum = pass * sums; ks0 < k_steps; ks0 += sum_steps, sum++) {
+            if (sum > 0 && ok && !mbar_wait_warp(&drained, (uint32_t)(sum - 1) & 1u, a.err)) ok = false;
             tc_fence_after();
-            const uint64_t dx = desc_plus(desc0, (uint32_t)(at * shape.stage_bytes));
-            for (int e = 0; e < n; e++) {
-                const uint64_t db = desc_plus(dx, (uint32_t)(kXBytes + e * a_bytes));
-                const uint32_t d = d0 + (uint32_t)(e * n16);
+            for (int ks = ks0 + w; ks < min(ks0 + sum_steps, k_steps) && ok; ks += issuers) {
+                if (!mbar_wait_warp(&full[at], par, a.err)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t dx = desc_plus(desc0, (uint32_t)(at * shape.stage_bytes));
+                for (int e = 0; e < n; e++) {
+                    const uint64_t db = desc_plus(dx, (uint32_t)(kXBytes + e * a_bytes));
+                    const uint32_t d = d0 + (uint32_t)(e * n16);
 #pragma unroll
-                for (int kk = 0; kk < kStep / 16; kk++)
-                    umma_f16_if<false>(lead, d, desc_plus(dx, kk * 32), desc_plus(db, kk * 32), idesc, ks != w || kk != 0);
+                    for (int kk = 0; kk < kStep / 16; kk++)
+                        umma_f16_if<false>(lead, d, desc_plus(dx, kk * 32), desc_plus(db, kk * 32), idesc, ks != ks0 + w || kk != 0);
+                }
+                umma_commit_if<false>(lead, smem_u32(&empty[at]));
+                at += issuers;
+                if (at >= S) { at -= S; par ^= 1u; }
             }
-            umma_commit_if<false>(lead, smem_u32(&empty[at]));
-            at += issuers;
-            if (at >= S) { at -= S; par ^= 1u; }
+            umma_commit_if<false>(lead, smem_u32(&done));     // (also after an expired wait)
         }
-        umma_commit_if<false>(lead, smem_u32(&done));     // (also after an expired wait)
         odd ^= (uint32_t)((st + k_steps) / S) & 1u;
         st = (st + k_steps) % S;
     };
@@ -382,24 +406,35 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         for (int base = base0; base < n_here && !direct; base += stride, pass++) multiply(min(side, n_here - base), pass);
     } else {
         const uint32_t tmem = (uint32_t)uniform((int)tmem_slot);
-        const int parts = min(issuers, k_steps);
         // an adapter's share, masked, as fp16 and what the rounding left: a row per lane
         const int r = warp * 32 + lane;
         const bool real = local0 + r < n_rows;
         const int mine = row_slot[r];
+        // 16 columns of adapter e's sums: those of all issuers (the last sum may have fewer), and what came before
+        const uint32_t total = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(issuers * acc_cols);
+        auto sum_up = [&](int e, int c, int sum, float (&v)[16]) {
+            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * n16 + c);
+            const int parts = min(issuers, k_steps - sum * sum_steps);
+            tmem_ld16(from, v);
+            for (int w = 1; w < parts; w++) {
+                float x[16];
+                tmem_ld16(from + (uint32_t)(w * acc_cols), x);
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] += x[i];
+            }
+            if (sum > 0) {
+                float x[16];
+                tmem_ld16(total + (uint32_t)(e * n16 + c), x);
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] += x[i];
+            }
+        };
         auto store = [&](int e, int s) {
             const float sc = a.scale ? a.scale[slots[s]] : 1.f;
             __half* out = p.t + ((first_block + s) * p.tile + local0 + r) * t_columns(rank);
             for (int c = 0; c < rank; c += 16) {
-                const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(e * n16 + c);
                 float v[16];
-                tmem_ld16(from, v);
-                for (int w = 1; w < parts; w++) {
-                    float x[16];
-                    tmem_ld16(from + (uint32_t)(w * acc_cols), x);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] += x[i];
-                }
+                sum_up(e, c, sums - 1, v);
                 uint32_t hi[8], low[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -430,7 +465,22 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         }
         int pass = 0;
         for (int base = base0; base < n_here && !direct; base += stride, pass++) {
-            mbar_wait(&done, (uint32_t)pass & 1u, a.err);
+            for (int sum = 0; sum < sums - 1; sum++) {
+                mbar_wait(&done, (uint32_t)(pass * sums + sum) & 1u, a.err);
+                __syncwarp();
+                tc_fence_after();
+                if (warp * 32 < kRows)
+                    for (int e = 0; e < min(side, n_here - base); e++)
+                        for (int c = 0; c < rank; c += 16) {
+                            float v[16];
+                            sum_up(e, c, sum, v);
+                            tmem_st16(total + (uint32_t)(e * n16 + c), v);
+                        }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&drained);
+            }
+            mbar_wait(&done, (uint32_t)(pass * sums + sums - 1) & 1u, a.err);
             __syncwarp();
             tc_fence_after();
             if (warp * 32 < kRows)
@@ -481,9 +531,9 @@ static int launch_rows(const LoraArgs& a, const LoraPlan& p, const CUtensorMap* 
     long long ny = 296 / chunks;
     if (ny > most) ny = most;
     if (ny < 1) ny = 1;
-    ShrinkShape shape = shrink_shape(ROWS, p.rank);
+    ShrinkShape shape = shrink_shape(ROWS, p.rank, a.K / kStep, a.sums != 0);
     shape.x_bytes = x_rows * kStep * 2;
-    shape.direct = chunks * a.n_adapters <= kDirect;
+    shape.direct = chunks * a.n_adapters <= kDirect && shape.sums == 1;   // (sums are added once the plan is there)
     if (shape.direct) ny = a.n_adapters;
     kern<<<dim3((unsigned)chunks, (unsigned)ny), kThreads, shape.smem, st>>>(tx, ta, a, p, shape);
     return cudaPeekAtLastError() == cudaSuccess ? W2V_OK : W2V_ERR_LAUNCH;

@@ -102,7 +102,7 @@ extern "C" int w2v_gemm_q_lora(const void* A, long long lda, long long K, long l
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return W2V_ERR_TENSOR_MAP;
         const sg::LoraArgs a{reinterpret_cast<const __half*>(A), lda, (int)K, M, reinterpret_cast<const __half*>(lora_a),
-                             lora_scale, n_adapters, off, T, adapter, n_utt, err};
+                             lora_scale, n_adapters, off, T, adapter, n_utt, err, !f16};
         rc = sg::lora_shrink(a, lo.plan, nullptr, 0, st);
         if (rc) return rc;
     }

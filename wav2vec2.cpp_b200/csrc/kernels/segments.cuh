@@ -55,6 +55,7 @@ struct LoraArgs {
     const int* adapter;
     int n_utt;
     int* err;
+    int sums;              // the sums over K end every 512 (fp32 outputs: segment_gemm.cu)
 };
 
 constexpr int kGroup = 32;                                                     // ranks whose values stand together
