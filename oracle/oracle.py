@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 import os
 import subprocess
+import warnings
 from pathlib import Path
 
 import numpy as np
@@ -384,8 +385,11 @@ def _table_beam_search(lg: np.ndarray, blank: int, beam: int) -> list[int]:
 
 
 def ref_beam_search(logits, blank: int, beam: int) -> list[int]:
+    """The reference's own decoder; where its build is absent, the restatement
+    above, with a warning that says so."""
     lg = np.ascontiguousarray(logits, np.float32)
     if not ref_available():
+        warnings.warn("no build of the reference: its beam search is this module's restatement of it", stacklevel=2)
         return _table_beam_search(lg, blank, beam)
     T, V = lg.shape
     out = np.zeros(max(T, 1) + 1, np.int32)
