@@ -150,3 +150,16 @@ def test_both_sides_of_a_block_per_adapter(K, synth, weights, epi, M, n_adapters
     c.lb[3].fill_(float("inf"))
     c.call()
     c.check()
+
+
+@pytest.mark.parametrize("rank,Kd", [(72, 2112), (96, 1088), (128, 1088), (40, 1600)])
+@pytest.mark.parametrize("M", [15000, 25000])
+def test_long_sums_of_large_ranks_on_every_sm(K, synth, rank, Kd, M):
+    """Blocks of the first product whose accumulators and totals take all of an SM's tensor memory,
+    more of them than SMs; several adapters in turn in some."""
+    lens = [700] * 20 + [1] * 40 + [M - 14040]
+    c = Lora(K, synth, Segments(lens), [i % 9 - 1 for i in range(len(lens))], 72, Kd, rank, 8, "f16", EPI_F32)
+    assert c.seg.M == M
+    c.call()
+    c.call()
+    c.check()
