@@ -26,9 +26,10 @@
 //
 // Few rows (kDirect): what counts is the way from the launch to the results.
 // Each adapter has a block of its own whether the rows use it or not, which loads and
-// multiplies before the plan is there.  Projections with adapters, the whole call
-// (one warp and the plan first -> these two): 16 single frames of 8 adapters, K = N = 1024,
-// 15.0 -> 13.1 us; 499 rows, K = N = 768, 4 adapters 12.3 -> 10.6 us.
+// multiplies before the plan is there.  Projections with adapters, the whole call from a short
+// graph: 16 single frames of 8 adapters, K = N = 1024, 13.2 us (one warp, and the plan first:
+// 1.9 more); 499 rows, K = N = 768, 4 adapters 10.3 (1.7 more).  Call after call the host's issue
+// of the two launches is more than that, 15.7 and 14.4 us.
 #include "segments.cuh"
 #include "w2v_kernels.h"
 

@@ -34,11 +34,13 @@
 // host and no workspace is needed); rows past the utterance are computed and
 // not stored.
 //
-// Bound: many rows by the MMAs and their operands' way from L2 under the power limit,
-// few rows by the launches and the dependent waits.  31936 rows, K 768, N 2304,
-// rank 16: 104 us, 1.11 PFLOP/s; 31.7 K rows, 1024 x 4096, rank 32, GELU: 224 us, 1.22;
-// 32 experts of 0 .. 1100 rows, 1024 x 4096, GELU: 152 us, 0.94 (the tiles' rows past the
-// utterances' ends not counted); 8 heads of 5 .. 49 rows, 768 x 48: 7.6 us.
+// Bound: many rows by the MMAs (the tensor pipe is busy 72 to 85 % of the cycles, the ways
+// from L2 at 38 to 42 % of their peak), few rows by the launches and the dependent waits.
+// From a short graph (in brackets: call after call for some time, at the clock that the power
+// limit then leaves, or the host's issue): 31936 rows, K 768, N 2304, rank 16: 105 us (125),
+// 1.10 PFLOP/s; 31.7 K rows, 1024 x 4096, rank 32, GELU: 224 us (264), 1.22; 32 experts of
+// 0 .. 1100 rows, 1024 x 4096, GELU: 150 us (182), 0.95 (the tiles' rows past the utterances'
+// ends not counted); 8 heads of 5 .. 49 rows, 768 x 48: 7.6 us (10.1).
 #include <algorithm>
 
 #include "segments.cuh"
@@ -663,8 +665,8 @@ static int launch_epi(int epi, const Maps& m, const Params& p, int tiles, bool d
 // Tile: width w (a multiple of 32) and single CTAs or pairs, by waves over the
 // SMs x the cycles of a tile.  A K-block of 64 takes an SM 2 w cycles of MMA; its
 // operands, 16 KB of rows and 128 w bytes of weights (half of that in a pair, which
-// shares them), come in at some 64 bytes a cycle.  A wave also has a fill, a
-// drain and an epilogue.
+// shares them), are counted at 64 bytes a cycle (a model, which orders the widths: the
+// path itself takes about twice as much).  A wave also has a fill, a drain and an epilogue.
 static void pick_tile(int N, long long m_tiles1, long long m_tiles2, long long K, int* bn, bool* pair) {
     double best = 1e300;
     for (int pr = 0; pr < 2; pr++)
