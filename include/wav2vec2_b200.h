@@ -84,7 +84,8 @@ int wav2vec2_b200_device_outputs(struct wav2vec2_context * ctx, const float ** l
  * Without such a batch (no forward_device yet, or one that failed) there is
  * nothing to search and nothing is written.  After any other forward on the
  * context's first device (a host batch, debug_stages), whose buffers these
- * are, it is refused (W2V_STATUS_INVALID) until the next forward_device. */
+ * are, it is refused (W2V_STATUS_INVALID) until the next forward_device; so it
+ * is in a stream that is being captured (w2v_ctc_beam may be captured). */
 int wav2vec2_b200_beam_device(struct wav2vec2_context * ctx, int beam_width, int n_best, int * ids, long long cap,
                               int * n_ids, double * scores, void * stream);
 

@@ -117,22 +117,28 @@ def test_searches_and_forwards_on_several_streams(B, model_path, synth):
     m.close()
 
 
-def test_captured_search(B, model_path, synth):
-    """A search captured into a graph after one like it has run, replayed after another."""
+def test_not_in_a_captured_stream(B, model_path, synth):
+    """A replay would search at addresses and sizes of a batch that is gone; the capture goes on
+    without it, and the context searches as before."""
     m = B.Model(model_path("tiny", "q8_0", bias_std=0.02, gain_jitter=0.1))
     x = synth.make_audio(20000, 5)
     d = torch.from_numpy(x).cuda()
     torch.cuda.synchronize()
     m.forward_device(d.data_ptr(), [len(x)])
     a, b = Outputs(1, 2, 80), Outputs(1, 2, 80)
+    other = torch.zeros(4, device="cuda")
     torch.cuda.synchronize()
     a.search(m, 8)
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
-        b.search(m, 8, torch.cuda.current_stream().cuda_stream)
+        other += 1
+        with pytest.raises(B.EngineError, match="captured"):
+            b.search(m, 8, torch.cuda.current_stream().cuda_stream)
     g.replay()
-    g.replay()
+    torch.cuda.synchronize()
+    assert b.untouched() and (other == 1).all()
+    b.search(m, 8)
     assert same(a.host(), b.host())
     m.close()
 

@@ -514,11 +514,10 @@ int wav2vec2_b200_beam_device(wav2vec2_context* ctx, int beam_width, int n_best,
         return W2V_STATUS_INVALID;
     }
     try {
-        Engine* e = ctx->engines[0].get();
-        if (!e->beam(beam_width, n_best, ids, cap, n_ids, scores, reinterpret_cast<cudaStream_t>(stream))) {
-            set_error(e->held_lost() ? "another forward has replaced the last device batch's logits" : "invalid arguments");
-            return W2V_STATUS_INVALID;
-        }
+        ctx->engines[0]->beam(beam_width, n_best, ids, cap, n_ids, scores, reinterpret_cast<cudaStream_t>(stream));
+    } catch (const std::invalid_argument& ex) {
+        set_error(ex.what());
+        return W2V_STATUS_INVALID;
     } catch (const std::exception& ex) {
         set_error(ex.what());
         return W2V_STATUS_CUDA;

@@ -520,27 +520,27 @@ static bool capturing(cudaStream_t st) {
     return s != cudaStreamCaptureStatusNone;
 }
 
-bool Engine::beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st) {
+void Engine::beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st) {
     cuda_check(cudaSetDevice(device_), "cudaSetDevice");
     if (!st) st = stream_;
     const int frames = std::max(held_T_max_, 1);
     const long long bytes = w2v_ctc_beam_state_bytes(held_n_utt_, cfg_.vocab, width, frames);
-    if (bytes < 0 || n_best < 1 || n_best > width || !ids || !n_ids || !scores || cap < 1 || held_lost_) return false;
-    if (held_n_utt_ == 0) return true;
+    if (bytes < 0 || n_best < 1 || n_best > width || !ids || !n_ids || !scores || cap < 1)
+        throw std::invalid_argument("invalid arguments");
+    if (held_lost_) throw std::invalid_argument("another forward has replaced the last device batch's logits");
+    // a graph would keep the buffers' addresses and the batch's sizes, which the next forward changes
+    if (capturing(st)) throw std::invalid_argument("the stream is being captured");
+    if (held_n_utt_ == 0) return;
     beam_state_.ensure((size_t)bytes);
     wait_for_beam(st);
     const int rc = w2v_ctc_beam(logits_.as<float>(), d_T_off_, d_T_, held_n_utt_, cfg_.vocab, cfg_.pad_id, width, frames, 0,
                                 beam_state_.p, bytes, n_best, ids, cap, n_ids, scores, err_.as<int>(), st);
-    if (rc == W2V_ERR_ARGS) return false;
+    if (rc == W2V_ERR_ARGS) throw std::invalid_argument("invalid arguments");
     if (rc != W2V_OK) throw std::runtime_error("ctc_beam: status " + std::to_string(rc));
-    if (!capturing(st)) {
-        cuda_check(cudaEventRecord(beam_done_, st), "beam event");
-        beam_pending_ = true;
-    }
-    return true;
+    cuda_check(cudaEventRecord(beam_done_, st), "beam event");
+    beam_pending_ = true;
 }
 
-// (A search in a stream that is being captured is ordered by whoever replays it.)
 void Engine::wait_for_beam(cudaStream_t st) {
     if (beam_pending_ && !capturing(st)) cuda_check(cudaStreamWaitEvent(st, beam_done_, 0), "beam wait");
 }

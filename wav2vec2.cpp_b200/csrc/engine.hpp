@@ -111,10 +111,9 @@ public:
     // forward() for a caller that keeps the outputs on the device: the batch that beam() searches.
     void forward_device(const float* d_audio, const BatchGeom& g, cudaStream_t st);
     // Prefix beam search on the logits of the last forward_device (outputs on
-    // the device, as w2v_ctc_beam's); false: sizes that it does not take, or
-    // another forward has taken the buffers since.
-    bool beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st);
-    bool held_lost() const { return held_lost_; }
+    // the device, as w2v_ctc_beam's).  std::invalid_argument: sizes that it does not
+    // take, a stream that is being captured, or another forward has taken the buffers since.
+    void beam(int width, int n_best, int* ids, long long cap, int* n_ids, double* scores, cudaStream_t st);
 
     // Device error word set by kernels whose bounded waits expired.
     int check_device_error();
